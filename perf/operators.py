@@ -326,13 +326,14 @@ def work(case):
 
 
 def _planned(s):
-    """The plan by its definition, request after request."""
-    page, table, free = s["case"]["page"], s["table"].tolist(), s["free"].tolist()
+    """The plan by its definition, request after request: the first that finds too few pages ends the giving."""
+    page, table, free, short = s["case"]["page"], s["table"].tolist(), s["free"].tolist(), False
     slots, positions, cu, lens, status, held = [], [], [0], [], [], []
     for r, (a, b) in enumerate(zip(s["lengths"].tolist(), s["new"].tolist())):
         fits = a + b <= len(table[r]) * page
         want = range(_pages(a, page), _pages(a + b, page)) if fits else range(0)
-        ok = fits and len(want) <= len(free)
+        short = short or len(want) > len(free)
+        ok = fits and not (short and len(want))
         for i in want if ok else ():
             table[r][i] = free.pop()
         slots += [table[r][p // page] * page + p % page if ok else -1 for p in range(a, a + b)]
