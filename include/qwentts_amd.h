@@ -340,6 +340,101 @@ hipError_t qtts_cp_frame_shared(
     const void* text_rows, int* out_tokens, void* out_combined,
     int eos_id, int* done, const QttsSampling* sampling, int frame_step, hipStream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Paged key-value cache: operators for serving many streams from one pool of pages. No
+ * counterpart in the reference (one contiguous cache for one stream). A layer's cache is pages
+ * of page_size tokens; block_table[r * table_stride + i] is the page of request r's tokens
+ * i * page_size .. , and slot = page * page_size + place in the page. All of these take device
+ * pointers, allocate nothing, keep no state and may be captured into graphs; calls on different
+ * streams are independent as long as their outputs and workspaces are.
+ * ------------------------------------------------------------------------------------- */
+enum { QTTS_BF16 = 0, QTTS_F16 = 1 };
+
+/* One layer's pages. Element (page, head, place, channel) of K (and of V) is at page * page_stride +
+ * head * head_stride + place * slot_stride + channel; strides in elements, multiples of 8 (page and
+ * head strides up to 2^31 - 1 for a head, slot strides up to 2^24), k and v 16-byte aligned.
+ * page_size: a power of two, 16 .. 65536. head_dim: 64 or 128. */
+typedef struct QttsPagedCache {
+    void* k;
+    void* v;
+    int dtype;                    /* QTTS_BF16 or QTTS_F16 */
+    int num_pages, page_size, num_kv_heads, head_dim;
+    long long page_stride, head_stride, slot_stride;
+} QttsPagedCache;
+
+/* Pages, slots and positions for new tokens. Request b holds lengths[b] tokens and gets
+ * new_tokens[b] more (values below 0 count as 0); the tokens of all requests are packed in request
+ * order into arrays of total_tokens. Pages are taken from the top of the stack free_pages[0 ..
+ * *free_count) in request order; a request that finds too few ends the giving (none behind it
+ * overtakes it). page_size is a power of two up to 65536.
+ *   block_table       gets the new pages of granted requests (other entries stay)
+ *   slots, positions  [total_tokens]: slot and position of each token; -1 and the position it would
+ *                     have where the request is refused, -1 and 0 past the last request's tokens
+ *   cu_tokens         [n_requests + 1]: first token of each request
+ *   kv_lens           [n_requests]: tokens held with the new ones; 0 where refused
+ *   lengths_out       [n_requests]: the same, but unchanged where refused (may be lengths)
+ *   free_count_out    [1]: pages left (may be free_count)
+ *   status            [n_requests]: 0 granted, 1 too few free pages, 2 more tokens than the table row
+ *                     holds, 3 the tokens pass total_tokens */
+hipError_t qtts_paged_plan(
+    int n_requests, int table_width, long long table_stride, int page_size, int total_tokens,
+    const int* new_tokens, const int* lengths, int* block_table, const int* free_pages,
+    int free_capacity, const int* free_count, int* slots, int* positions, int* cu_tokens,
+    int* kv_lens, int* lengths_out, int* free_count_out, int* status, hipStream_t stream);
+
+/* The counterpart of a plan: requests with release[b] != 0 give their pages back to the stack, their
+ * lengths become 0 and those table entries -1. free_capacity: entries of free_pages. */
+hipError_t qtts_paged_release(
+    int n_requests, int table_width, long long table_stride, int page_size, const int* release,
+    int* lengths, int* block_table, int* free_pages, int free_capacity, int* free_count,
+    hipStream_t stream);
+
+/* RMSNorm of every query and key head (gain q_weight / k_weight [head_dim], NULL: no norm), rotation
+ * (halves d and d + head_dim / 2) and store: q_out [n_tokens, num_q_heads, head_dim], K (rotated) and V
+ * to the tokens' slots. Arithmetic in f32, one rounding. q, k, v and q_out are of the cache's type
+ * with strides of their own (elements, multiples of 8; q_out may be q); pointers are 16-byte
+ * aligned. cos / sin tables: [table_rows, head_dim], the halves of a row alike, of the cache's type
+ * or f32 (table_f32). positions: one row [n_tokens] (position_stride 0) or three, (t, h, w),
+ * position_stride apart: channel d of a half takes h if d % 3 == 1 and d < h_channels, w if d % 3 == 2
+ * and d < w_channels, else t; clamped into the table. A token whose slot is negative or past the
+ * pages is skipped: nothing of it is written, its query row included. Slots are distinct. */
+hipError_t qtts_qk_norm_rope_store(
+    const QttsPagedCache* cache, int n_tokens, int num_q_heads, const void* q,
+    long long q_token_stride, long long q_head_stride, const void* k, long long k_token_stride,
+    long long k_head_stride, const void* v, long long v_token_stride, long long v_head_stride,
+    void* q_out, long long out_token_stride, long long out_head_stride, const void* q_weight,
+    const void* k_weight, float eps, const void* cos_table, const void* sin_table, int table_f32,
+    int table_rows, const int* positions, long long position_stride, int h_channels, int w_channels,
+    const int* slots, hipStream_t stream);
+
+/* Attention of one new token per request, at position kv_lens[b] - 1, over the request's pages:
+ * softmax(scale q . k) v over the keys j < kv_lens[b]; with window > 0 only those with
+ * j >= kv_lens[b] - window or j < sinks. Query head h reads KV head h / (num_q_heads /
+ * num_kv_heads). A request of length 0 gets zeros, as does a query with no finite score; keys on
+ * pages outside [0, num_pages) are not seen; lengths are clamped to [0, table_width * page_size].
+ * max_len: the longest request as far as the caller knows (it sets how the keys are split; longer
+ * requests are computed too). scale > 0. The workspace of
+ * qtts_paged_decode_workspace_bytes() bytes (0: none is used), 16-byte aligned, needs no
+ * initialisation and is free again when the call's work on the stream is done. */
+size_t qtts_paged_decode_workspace_bytes(int n_requests, int num_q_heads, int num_kv_heads, int head_dim,
+                                         int table_width, int page_size, int max_len, int window, int sinks);
+hipError_t qtts_paged_attention_decode(
+    const QttsPagedCache* cache, int n_requests, int num_q_heads, const void* q,
+    long long q_token_stride, long long q_head_stride, void* out, long long out_token_stride,
+    long long out_head_stride, const int* block_table, int table_width, long long table_stride,
+    const int* kv_lens, int max_len, float scale, int window, int sinks, void* workspace,
+    size_t workspace_bytes, hipStream_t stream);
+
+/* The same for the new tokens of prompts: request b's are tokens cu_tokens[b] .. cu_tokens[b + 1] - 1
+ * of q and out, the last of them at position kv_lens[b] - 1; each sees the keys up to its own position
+ * (under a window as above, from its own position). Tokens before position 0 (kv_lens[b] below the
+ * request's tokens) get zeros; rows of out past the last request stay as they were. */
+hipError_t qtts_paged_attention_prefill(
+    const QttsPagedCache* cache, int n_requests, int n_tokens, int num_q_heads, const void* q,
+    long long q_token_stride, long long q_head_stride, void* out, long long out_token_stride,
+    long long out_head_stride, const int* block_table, int table_width, long long table_stride,
+    const int* kv_lens, const int* cu_tokens, float scale, int window, int sinks, hipStream_t stream);
+
 /* Debugging aid (no reference counterpart): record the weight-shared kernels' step timeline
  * (s_memrealtime stamps, [256 workgroups][1024 steps][16]: after the entry barrier, after the
  * partials barrier, the end of each of the 8 waves' vector work, 6 points inside a step) into

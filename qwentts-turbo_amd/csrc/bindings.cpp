@@ -11,7 +11,10 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <hip/hip_runtime_api.h>
+#include <algorithm>
+#include <climits>
 #include <cmath>
+#include <string>
 #include <vector>
 #include "qwentts_amd.h"
 
@@ -634,6 +637,246 @@ class MegakernelCodePredictorDecoder {
   torch::Tensor ws_shared_;                            // frames_streams(shared=True): the weight-shared launches' workspace
 };
 
+// ---------------------------------------------------------------------------------------
+// Paged-cache operators: functions over tensors (no reference counterpart).
+using torch::Tensor;
+using OptTensor = c10::optional<torch::Tensor>;
+
+const int* check_i32(const Tensor& t, const torch::Device& dev, int64_t n, const char* name) {
+  TORCH_CHECK(t.device() == dev, name, " must be on ", dev, ", got ", t.device());
+  TORCH_CHECK(t.scalar_type() == torch::kInt32 && t.is_contiguous(), name, " must be a contiguous int32 tensor");
+  TORCH_CHECK(t.numel() >= n, name, " needs ", n, " entries, got ", t.numel());
+  return t.data_ptr<int>();
+}
+
+void check_aligned(const Tensor& t, const char* name) {
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0, name, " must be 16-byte aligned");
+}
+
+// block_table [requests, width] int32, rows of its own stride
+void check_table(const Tensor& t, const torch::Device& dev, int64_t requests) {
+  TORCH_CHECK(t.device() == dev, "block_table must be on ", dev, ", got ", t.device());
+  TORCH_CHECK(t.scalar_type() == torch::kInt32 && t.dim() == 2 && t.size(0) >= requests && t.size(1) >= 1,
+              "block_table must be an int32 [requests, width] tensor with >= ", requests, " rows");
+  TORCH_CHECK(t.stride(1) == 1 || t.size(1) == 1, "block_table rows must be contiguous");
+  TORCH_CHECK(t.size(0) == 1 || t.stride(0) >= t.size(1), "block_table rows must not overlap");
+}
+long long table_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
+
+void check_page_size(int64_t page_size, int64_t least) {
+  TORCH_CHECK(page_size >= least && page_size <= 65536 && (page_size & (page_size - 1)) == 0,
+              "page_size must be a power of two in [", least, ", 65536], got ", page_size);
+}
+
+QttsPagedCache paged_cache(const Tensor& k, const Tensor& v) {
+  TORCH_CHECK(k.is_cuda(), "k_cache must be a GPU tensor");
+  TORCH_CHECK(k.scalar_type() == torch::kBFloat16 || k.scalar_type() == torch::kFloat16,
+              "the cache must be bfloat16 or float16, got ", k.scalar_type());
+  TORCH_CHECK(k.dim() == 4, "k_cache must be [pages, kv_heads, page_size, head_dim], got ", k.sizes());
+  TORCH_CHECK(v.device() == k.device() && v.scalar_type() == k.scalar_type() && v.sizes() == k.sizes() && v.strides() == k.strides(),
+              "v_cache must be like k_cache (device, type, shape and strides)");
+  TORCH_CHECK(k.size(3) == 64 || k.size(3) == 128, "head_dim must be 64 or 128, got ", k.size(3));
+  check_page_size(k.size(2), 16);
+  TORCH_CHECK(k.size(0) >= 1 && k.size(0) <= INT_MAX && k.size(1) >= 1 && k.size(1) <= INT_MAX, "empty cache: ", k.sizes());
+  TORCH_CHECK(k.stride(3) == 1, "the cache's channels must be contiguous");
+  for (int i = 0; i < 3; ++i) TORCH_CHECK(k.stride(i) >= 0 && k.stride(i) % 8 == 0, "cache strides must be multiples of 8, got ", k.strides());
+  TORCH_CHECK(k.stride(2) >= k.size(3) && k.stride(2) <= (1 << 24) && k.stride(1) <= INT_MAX, "cache strides out of range: ", k.strides());
+  check_aligned(k, "k_cache");
+  check_aligned(v, "v_cache");
+  QttsPagedCache c;
+  c.k = k.data_ptr();
+  c.v = v.data_ptr();
+  c.dtype = k.scalar_type() == torch::kBFloat16 ? QTTS_BF16 : QTTS_F16;
+  c.num_pages = (int)k.size(0);
+  c.num_kv_heads = (int)k.size(1);
+  c.page_size = (int)k.size(2);
+  c.head_dim = (int)k.size(3);
+  c.page_stride = k.stride(0);
+  c.head_stride = k.stride(1);
+  c.slot_stride = k.stride(2);
+  return c;
+}
+
+// [tokens, heads, head_dim] of the cache's type; channels contiguous, the other strides multiples of 8
+void check_heads(const Tensor& t, const Tensor& cache, int64_t tokens, int64_t heads, const char* name) {
+  TORCH_CHECK(t.device() == cache.device(), name, " must be on ", cache.device(), ", got ", t.device());
+  TORCH_CHECK(t.scalar_type() == cache.scalar_type(), name, " must be of the cache's type ", cache.scalar_type(), ", got ", t.scalar_type());
+  TORCH_CHECK(t.dim() == 3 && t.size(0) == tokens && (heads < 0 || t.size(1) == heads) && t.size(1) >= 1 && t.size(2) == cache.size(3),
+              name, " must be [", tokens, ", ", heads < 0 ? std::string("heads") : std::to_string(heads), ", ", cache.size(3), "], got ", t.sizes());
+  if (t.numel() == 0) return;
+  TORCH_CHECK(t.stride(2) == 1, name, ": channels must be contiguous");
+  TORCH_CHECK((t.size(0) == 1 || t.stride(0) % 8 == 0) && (t.size(1) == 1 || t.stride(1) % 8 == 0), name,
+              ": token and head strides must be multiples of 8, got ", t.strides());
+  check_aligned(t, name);
+}
+long long tok_stride(const Tensor& t) { return t.size(0) == 1 ? 0 : t.stride(0); }
+long long head_stride(const Tensor& t) { return t.size(1) == 1 ? 0 : t.stride(1); }
+
+std::vector<Tensor> paged_plan(Tensor new_tokens, Tensor lengths, Tensor block_table, Tensor free_pages, Tensor free_count,
+                               int64_t page_size, int64_t total_tokens, OptTensor lengths_out, OptTensor free_count_out) {
+  TORCH_CHECK(new_tokens.is_cuda(), "new_tokens must be a GPU tensor");
+  const torch::Device dev = new_tokens.device();
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  const int64_t n = new_tokens.numel();
+  TORCH_CHECK(n >= 1 && n <= INT_MAX, "a plan needs at least one request");
+  TORCH_CHECK(total_tokens >= 0 && total_tokens <= INT_MAX, "total_tokens out of range: ", total_tokens);
+  const int* nt = check_i32(new_tokens, dev, n, "new_tokens");
+  int* len = const_cast<int*>(check_i32(lengths, dev, n, "lengths"));
+  check_table(block_table, dev, n);
+  const int* fp = check_i32(free_pages, dev, 0, "free_pages");
+  int* fc = const_cast<int*>(check_i32(free_count, dev, 1, "free_count"));
+  check_page_size(page_size, 1);
+  TORCH_CHECK(block_table.size(1) <= INT_MAX / page_size, "a block_table row holds more than 2^31 - 1 tokens");
+  int* len_out = lengths_out.has_value() ? const_cast<int*>(check_i32(*lengths_out, dev, n, "lengths_out")) : len;
+  int* fc_out = free_count_out.has_value() ? const_cast<int*>(check_i32(*free_count_out, dev, 1, "free_count_out")) : fc;
+  auto i32 = torch::dtype(torch::kInt32).device(dev);
+  auto slots = torch::empty({total_tokens}, i32), positions = torch::empty({total_tokens}, i32);
+  auto cu = torch::empty({n + 1}, i32), kv = torch::empty({n}, i32), status = torch::empty({n}, i32);
+  hip_check(qtts_paged_plan((int)n, (int)block_table.size(1), table_stride(block_table), (int)page_size, (int)total_tokens, nt, len,
+                            block_table.data_ptr<int>(), fp, (int)std::min<int64_t>(free_pages.numel(), INT_MAX), fc,
+                            slots.data_ptr<int>(), positions.data_ptr<int>(), cu.data_ptr<int>(), kv.data_ptr<int>(), len_out,
+                            fc_out, status.data_ptr<int>(), cur_stream()),
+            "qtts_paged_plan");
+  return {slots, positions, cu, kv, status};
+}
+
+void paged_release(Tensor release, Tensor lengths, Tensor block_table, Tensor free_pages, Tensor free_count, int64_t page_size) {
+  TORCH_CHECK(release.is_cuda(), "release must be a GPU tensor");
+  const torch::Device dev = release.device();
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  const int64_t n = release.numel();
+  TORCH_CHECK(n >= 1 && n <= INT_MAX, "a release needs at least one request");
+  const int* rel = check_i32(release, dev, n, "release");
+  check_i32(lengths, dev, n, "lengths");
+  check_table(block_table, dev, n);
+  check_i32(free_pages, dev, 1, "free_pages");
+  check_i32(free_count, dev, 1, "free_count");
+  check_page_size(page_size, 1);
+  hip_check(qtts_paged_release((int)n, (int)block_table.size(1), table_stride(block_table), (int)page_size, rel,
+                               lengths.data_ptr<int>(), block_table.data_ptr<int>(), free_pages.data_ptr<int>(),
+                               (int)std::min<int64_t>(free_pages.numel(), INT_MAX), free_count.data_ptr<int>(), cur_stream()),
+            "qtts_paged_release");
+}
+
+Tensor qk_norm_rope_store(Tensor q, Tensor k, Tensor v, OptTensor q_weight, OptTensor k_weight, Tensor cos_table, Tensor sin_table,
+                          Tensor positions, Tensor slots, Tensor k_cache, Tensor v_cache, double eps,
+                          std::vector<int64_t> mrope_section, OptTensor out) {
+  const QttsPagedCache cache = paged_cache(k_cache, v_cache);
+  const torch::Device dev = k_cache.device();
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  const int64_t n = q.dim() == 3 ? q.size(0) : -1, dim = cache.head_dim;
+  TORCH_CHECK(n >= 0 && n <= INT_MAX, "q must be [tokens, heads, head_dim], got ", q.sizes());
+  check_heads(q, k_cache, n, -1, "q");
+  check_heads(k, k_cache, n, cache.num_kv_heads, "k");
+  check_heads(v, k_cache, n, cache.num_kv_heads, "v");
+  TORCH_CHECK(q.size(1) <= INT_MAX, "too many heads");
+  for (const OptTensor* w : {&q_weight, &k_weight})
+    if (w->has_value()) {
+      TORCH_CHECK((*w)->device() == dev && (*w)->scalar_type() == k_cache.scalar_type() && (*w)->is_contiguous() && (*w)->dim() == 1 &&
+                      (*w)->size(0) == dim, "norm weights must be contiguous [", dim, "] tensors of the cache's type on ", dev);
+      check_aligned(**w, "norm weights");
+    }
+  TORCH_CHECK(cos_table.device() == dev && cos_table.dim() == 2 && cos_table.size(0) >= 1 && cos_table.size(0) <= INT_MAX &&
+                  cos_table.size(1) == dim && cos_table.is_contiguous(), "cos must be a contiguous [rows, ", dim, "] tensor on ", dev);
+  TORCH_CHECK(cos_table.scalar_type() == k_cache.scalar_type() || cos_table.scalar_type() == torch::kFloat32,
+              "cos and sin must be of the cache's type or float32");
+  TORCH_CHECK(sin_table.device() == dev && sin_table.scalar_type() == cos_table.scalar_type() && sin_table.sizes() == cos_table.sizes() &&
+                  sin_table.is_contiguous(), "sin must be like cos");
+  check_aligned(cos_table, "cos");
+  check_aligned(sin_table, "sin");
+  const bool three = positions.dim() == 2;
+  TORCH_CHECK((positions.dim() == 1 && positions.size(0) == n) || (three && positions.size(0) == 3 && positions.size(1) == n),
+              "positions must be [", n, "] or [3, ", n, "], got ", positions.sizes());
+  const int* pos = check_i32(positions, dev, n, "positions");
+  const int* slot = check_i32(slots, dev, n, "slots");
+  TORCH_CHECK(slots.numel() == n, "slots must have one entry per token");
+  int64_t h = 0, w = 0;
+  if (three) {
+    TORCH_CHECK(mrope_section.size() == 3 && mrope_section[0] >= 0 && mrope_section[1] >= 0 && mrope_section[2] >= 0 &&
+                    mrope_section[0] + mrope_section[1] + mrope_section[2] == dim / 2,
+                "mrope_section must be three counts that add up to head_dim / 2 = ", dim / 2);
+    h = 3 * mrope_section[1];
+    w = 3 * mrope_section[2];
+    TORCH_CHECK(h <= dim / 2 && w <= dim / 2, "mrope_section: h and w take at most a third of the channels each");
+  }
+  TORCH_CHECK(eps >= 0.0, "eps must be >= 0");
+  Tensor o;
+  if (out.has_value()) {
+    o = *out;
+    check_heads(o, k_cache, n, q.size(1), "out");
+  } else {
+    o = torch::empty({n, q.size(1), dim}, q.options());
+  }
+  if (n == 0) return o;
+  hip_check(qtts_qk_norm_rope_store(&cache, (int)n, (int)q.size(1), q.data_ptr(), tok_stride(q), head_stride(q), k.data_ptr(),
+                                    tok_stride(k), head_stride(k), v.data_ptr(), tok_stride(v), head_stride(v), o.data_ptr(),
+                                    tok_stride(o), head_stride(o), q_weight.has_value() ? q_weight->data_ptr() : nullptr,
+                                    k_weight.has_value() ? k_weight->data_ptr() : nullptr, (float)eps, cos_table.data_ptr(),
+                                    sin_table.data_ptr(), cos_table.scalar_type() == torch::kFloat32, (int)cos_table.size(0), pos,
+                                    three ? n : 0, (int)h, (int)w, slot, cur_stream()),
+            "qtts_qk_norm_rope_store");
+  return o;
+}
+
+// what both attention calls check: returns the output tensor
+Tensor check_attention(const QttsPagedCache& cache, const Tensor& q, const Tensor& k_cache, const Tensor& block_table,
+                       const Tensor& kv_lens, int64_t requests, double scale, int64_t window, int64_t sinks, OptTensor out) {
+  const torch::Device dev = k_cache.device();
+  TORCH_CHECK(q.dim() == 3, "q must be [tokens, heads, head_dim], got ", q.sizes());
+  check_heads(q, k_cache, q.size(0), -1, "q");
+  TORCH_CHECK(q.size(1) % cache.num_kv_heads == 0, "q's heads (", q.size(1), ") must be a multiple of the cache's (", cache.num_kv_heads, ")");
+  TORCH_CHECK(q.size(0) * q.size(1) <= INT_MAX / 2, "q has too many rows");
+  TORCH_CHECK(requests >= 1 && requests <= INT_MAX, "at least one request is needed");
+  check_table(block_table, dev, requests);
+  TORCH_CHECK(block_table.size(1) <= (INT_MAX - 4096) / cache.page_size, "a block_table row holds more than 2^31 - 4097 tokens");
+  check_i32(kv_lens, dev, requests, "kv_lens");
+  TORCH_CHECK(scale > 0.0 && std::isfinite((float)scale) && (float)scale > 0.0f, "scale must be positive and finite");
+  TORCH_CHECK(window >= 0 && window <= INT_MAX && sinks >= 0 && sinks <= INT_MAX, "window and sinks must be >= 0");
+  if (!out.has_value()) return torch::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  check_heads(*out, k_cache, q.size(0), q.size(1), "out");
+  return *out;
+}
+
+Tensor paged_attention_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor kv_lens, double scale,
+                              int64_t window, int64_t sinks, int64_t max_len, OptTensor out) {
+  const QttsPagedCache cache = paged_cache(k_cache, v_cache);
+  const torch::Device dev = k_cache.device();
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  const int64_t n = q.dim() == 3 ? q.size(0) : 0;
+  Tensor o = check_attention(cache, q, k_cache, block_table, kv_lens, n, scale, window, sinks, out);
+  const int width = (int)block_table.size(1);
+  TORCH_CHECK(max_len >= 1, "max_len must be >= 1");
+  const int most = (int)std::min<int64_t>(max_len, (int64_t)width * cache.page_size);
+  const size_t need = qtts_paged_decode_workspace_bytes((int)n, (int)q.size(1), cache.num_kv_heads, cache.head_dim, width,
+                                                        cache.page_size, most, (int)window, (int)sinks);
+  Tensor ws;
+  if (need > 0) ws = torch::empty({(int64_t)need}, torch::dtype(torch::kUInt8).device(dev));
+  hip_check(qtts_paged_attention_decode(&cache, (int)n, (int)q.size(1), q.data_ptr(), tok_stride(q), head_stride(q), o.data_ptr(),
+                                        tok_stride(o), head_stride(o), block_table.data_ptr<int>(), width, table_stride(block_table),
+                                        kv_lens.data_ptr<int>(), most, (float)scale, (int)window, (int)sinks,
+                                        need > 0 ? ws.data_ptr() : nullptr, need, cur_stream()),
+            "qtts_paged_attention_decode");
+  return o;
+}
+
+Tensor paged_attention_prefill(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor kv_lens, Tensor cu_tokens,
+                               double scale, int64_t window, int64_t sinks, int64_t max_len, OptTensor out) {
+  const QttsPagedCache cache = paged_cache(k_cache, v_cache);
+  const torch::Device dev = k_cache.device();
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
+  TORCH_CHECK(max_len >= 1, "max_len must be >= 1");
+  const int64_t n = cu_tokens.numel() - 1;
+  Tensor o = check_attention(cache, q, k_cache, block_table, kv_lens, n, scale, window, sinks, out);
+  const int* cu = check_i32(cu_tokens, dev, n + 1, "cu_tokens");
+  if (q.size(0) == 0) return o;
+  hip_check(qtts_paged_attention_prefill(&cache, (int)n, (int)q.size(0), (int)q.size(1), q.data_ptr(), tok_stride(q), head_stride(q),
+                                         o.data_ptr(), tok_stride(o), head_stride(o), block_table.data_ptr<int>(),
+                                         (int)block_table.size(1), table_stride(block_table), kv_lens.data_ptr<int>(), cu,
+                                         (float)scale, (int)window, (int)sinks, cur_stream()),
+            "qtts_paged_attention_prefill");
+  return o;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_qwentts_amd_C, m) {
@@ -651,6 +894,20 @@ PYBIND11_MODULE(_qwentts_amd_C, m) {
     TORCH_CHECK(buf->is_cuda() && buf->is_contiguous(), "trace buffer must be a contiguous GPU tensor");
     hip_check(qtts_debug_trace_shared(buf->data_ptr(), (size_t)buf->numel() * buf->element_size()), "qtts_debug_trace_shared");
   }, py::arg("buffer") = py::none());
+  m.def("paged_plan", &paged_plan, py::arg("new_tokens"), py::arg("lengths"), py::arg("block_table"), py::arg("free_pages"),
+        py::arg("free_count"), py::arg("page_size"), py::arg("total_tokens"), py::arg("lengths_out") = py::none(),
+        py::arg("free_count_out") = py::none());
+  m.def("paged_release", &paged_release, py::arg("release"), py::arg("lengths"), py::arg("block_table"), py::arg("free_pages"),
+        py::arg("free_count"), py::arg("page_size"));
+  m.def("qk_norm_rope_store", &qk_norm_rope_store, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("q_weight"), py::arg("k_weight"),
+        py::arg("cos"), py::arg("sin"), py::arg("positions"), py::arg("slots"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("eps"), py::arg("mrope_section"), py::arg("out") = py::none());
+  m.def("paged_attention_decode", &paged_attention_decode, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("block_table"), py::arg("kv_lens"), py::arg("scale"), py::arg("window"), py::arg("sinks"), py::arg("max_len"),
+        py::arg("out") = py::none());
+  m.def("paged_attention_prefill", &paged_attention_prefill, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("block_table"), py::arg("kv_lens"), py::arg("cu_tokens"), py::arg("scale"), py::arg("window"), py::arg("sinks"),
+        py::arg("max_len"), py::arg("out") = py::none());
   py::class_<MegakernelTTSDecoder>(m, "MegakernelTTSDecoder")
       .def(py::init<torch::Tensor, std::vector<torch::Tensor>, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor,
                     int64_t, int64_t>())

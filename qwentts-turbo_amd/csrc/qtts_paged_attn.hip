@@ -1,0 +1,803 @@
+// Attention over a paged key-value cache on MI355X (gfx950): one new token per request (decode), and the
+// new tokens of prompts (prefill). The cache's layout is in qtts_paged.hip.
+//
+//   o = sum_j w_j v_j / sum_j w_j,  w_j = e^(scale q . k_j - max),  over the keys j that the query sees:
+//   j <= p (its position) and, under a window of w keys, j > p - w or j < sinks.
+// A query that sees no key (or no finite score) gets zeros. Keys that no query of a workgroup sees are
+// never loaded as numbers: their rows come as zeros, so what unused slots hold (NaN included) does not
+// matter. A key on a page outside the cache (an entry of -1) is not seen.
+#include "qtts_paged.h"
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+namespace qtts {
+namespace pg {
+
+typedef __attribute__((address_space(3))) void lvoid_t;
+
+// Wait until at most N of this wave's vector-memory instructions and none of its LDS reads are in flight.
+template <int N>
+__device__ __forceinline__ void wait_vm_lds() {
+  static_assert(N >= 0 && N <= 63, "vmcnt field");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
+}
+
+struct AttnArgs {
+  const uint16_t* q;
+  uint16_t* out;
+  long long q_token, q_head, o_token, o_head;    // strides in elements
+  Pages pages;
+  const int* table;
+  long long table_stride;
+  int width;                                     // table entries of a request
+  const int* lens;
+  const int* cu;                                 // prefill: first token of each request
+  int requests, tokens, hq, hkv, group;          // group: query heads of a KV head
+  float scale_log2;                              // scale * log2(e)
+  int window, sinks;                             // window 0: none
+  int splits, blocks;                            // decode: most units of a request, blocks a unit
+  float* part;                                   // [requests][hq][splits][D] sums
+  float* part_ml;                                // [requests][hq][splits][2] running max and sum
+};
+
+// A request's keys, clamped to what its table can hold.
+__device__ __forceinline__ int request_len(const AttnArgs& g, int b) {
+  const long long most = (long long)g.width << g.pages.shift;
+  return (int)min((long long)max(ld_const(g.lens + b), 0), most);
+}
+
+// The blocks of KB keys that a range of queries reads: those of the first `sinks` keys, then those from the
+// first key of the lowest window (lo) to the last key. t-th block: t < ns ? t : t + skip.
+struct Blocks {
+  int ns, skip, n;
+};
+template <int KB>
+__device__ __forceinline__ Blocks blocks_of(int lo, int end, int sinks) {
+  Blocks r;
+  const int first = lo / KB;
+  r.ns = (int)min((long long)first, ((long long)min(sinks, lo) + KB - 1) / KB);
+  r.skip = first - r.ns;
+  r.n = (end + KB - 1) / KB - r.skip;
+  return r;
+}
+
+// One 16-key piece of K and V into LDS by DMA, row r at r * 2 D bytes with its 16-byte chunk c at position
+// c ^ (r & 7). The descriptors begin at the piece's first row and end with its last, and rows that are
+// not `seen` are asked for past the end: they come as zeros.
+template <int D, class Seen>
+__device__ __forceinline__ void copy_piece(const Pages& pg, int page, int key0, int kvh, char* k_dst, char* v_dst, int lane,
+                                           Seen&& seen) {
+  constexpr int CPR = D / 8, RPI = 64 / CPR;           // chunks a row, rows an instruction
+  const long long at = (long long)page * pg.page_stride + (long long)kvh * pg.head_stride +
+                       (long long)(key0 & ((1 << pg.shift) - 1)) * pg.slot_stride;
+  const int bytes = (15 * pg.slot_stride + D) * 2;
+  const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(pg.k + at), (short)0, bytes, 0x00020000);
+  const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(pg.v + at), (short)0, bytes, 0x00020000);
+#pragma unroll
+  for (int i = 0; i < 16 / RPI; ++i) {
+    const int r = RPI * i + lane / CPR;
+    const int in = r * pg.slot_stride * 2 + ((lane % CPR) ^ (r & 7)) * 16;
+    const int off = seen(key0 + r) ? in : 0x7fffff00;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lvoid_t*)(k_dst + i * 1024), 16, off, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lvoid_t*)(v_dst + i * 1024), 16, off, 0, 0, 0);
+  }
+}
+
+// ---- decode --------------------------------------------------------------------------------
+// One workgroup of 4 waves per (request, KV head, up to 16 of its query heads, part of its keys). Bound by
+// reading K and V: every wave streams its own 32-key blocks (blocks w, w + 4, .. of the unit) through two
+// LDS buffers of its own, so the loop has no barrier, and 64 KB or more a CU are in flight.
+//   S^T = K Q^T on MFMA 16x16x32 (A: 16 keys x 32 channels from LDS, B: Q^T in registers): lane (g, c) holds
+//     head c's scores of keys 4 g + r and 16 + 4 g + r, r < 4; the max over a head's keys is in-lane and two
+//     exchanges.
+//   O^T += V^T P^T: P^T is the score registers as they are (k-index 8 g + j is key 4 g + j for j < 4 and
+//     16 + 4 g + j - 4 above), V^T comes through LDS transpose reads of 4 keys each. P goes in as two 16-bit
+//     numbers, the rounded value and the rounded rest, so that its rounding is that of 16 bits or more: the
+//     matrix units are idle otherwise.
+// The heads of a group share every K and V byte; a group over 16 is several workgroups. The 4 waves join
+// through LDS, the units of a request through part / part_ml and decode_join_kernel, both in key order, so
+// results do not depend on timing. A request of one unit writes its output here.
+constexpr int DW = 4;                 // waves
+constexpr int DKB = 32;               // keys of a block
+
+// The transpose reads of an MFMA step: 4 keys at LDS addresses a[0..3] + OFF and 4 more T bytes further, of
+// each channel block. In assembly with their wait: before the builtin the compiler waits for every DMA in
+// flight, the next block's among them.
+template <int OFF, int T>
+__device__ __forceinline__ void tr_read8(const uint32_t (&a)[4], u32x2 (&lo)[4], u32x2 (&hi)[4]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %8 offset:%c12\n\tds_read_b64_tr_b16 %4, %8 offset:%c13\n\t"
+      "ds_read_b64_tr_b16 %1, %9 offset:%c12\n\tds_read_b64_tr_b16 %5, %9 offset:%c13\n\t"
+      "ds_read_b64_tr_b16 %2, %10 offset:%c12\n\tds_read_b64_tr_b16 %6, %10 offset:%c13\n\t"
+      "ds_read_b64_tr_b16 %3, %11 offset:%c12\n\tds_read_b64_tr_b16 %7, %11 offset:%c13\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(lo[2]), "=&v"(lo[3]), "=&v"(hi[0]), "=&v"(hi[1]), "=&v"(hi[2]), "=&v"(hi[3])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "i"(OFF), "i"(OFF + T)
+      : "memory");
+}
+
+template <int OFF, int T>
+__device__ __forceinline__ void tr_read4(const uint32_t (&a)[4], u32x2 (&lo)[4], u32x2 (&hi)[4]) {
+  asm volatile(
+      "ds_read_b64_tr_b16 %0, %4 offset:%c6\n\tds_read_b64_tr_b16 %2, %4 offset:%c7\n\t"
+      "ds_read_b64_tr_b16 %1, %5 offset:%c6\n\tds_read_b64_tr_b16 %3, %5 offset:%c7\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(hi[0]), "=&v"(hi[1])
+      : "v"(a[0]), "v"(a[1]), "i"(OFF), "i"(OFF + T)
+      : "memory");
+}
+
+template <class E, int D>
+__global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
+  constexpr int BLK = DKB * D * 2;               // bytes of a K or V block
+  constexpr int MB = D / 16, KS = D / 32;        // 16-channel blocks of O^T, MFMA steps of a score
+  constexpr int NL = 2 * DKB * D * 2 / 1024;     // DMA instructions of a block
+  __shared__ __attribute__((aligned(1024))) char smem[DW * 4 * BLK];   // (K, V) x 2 buffers a wave
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int c = lane & 15, gr = lane >> 4;
+  int id = blockIdx.x;
+  const int kvh = id % g.hkv; id /= g.hkv;
+  const int unit = id % g.splits; id /= g.splits;
+  const int tiles = (g.group + 15) / 16, tile = id % tiles, b = id / tiles;
+  const int head0 = kvh * g.group + 16 * tile, nh = min(16, g.group - 16 * tile);
+
+  const int len = request_len(g, b);
+  const int lo = g.window > 0 ? max(len - g.window, 0) : 0;
+  const Blocks bl = blocks_of<DKB>(lo, len, g.sinks);
+  // a unit is g.blocks blocks, or more where the request is longer than the caller said
+  const int per = max(g.blocks, (bl.n + g.splits - 1) / g.splits);
+  const int units = max(1, (bl.n + per - 1) / per);
+  if (unit >= units) return;
+  const int t1 = min(bl.n, (unit + 1) * per), t0 = unit * per + w;
+  const int nt = t0 < t1 ? (t1 - t0 + DW - 1) / DW : 0;   // this wave's blocks
+
+  // Q^T: head c, channels 32 s + 8 gr ..
+  u32x4 q[KS];
+  const uint16_t* qp = g.q + (long long)b * g.q_token + (long long)(head0 + min(c, nh - 1)) * g.q_head + 8 * gr;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) q[s] = ldw(qp + 32 * s);
+
+  char* const buf = smem + w * 4 * BLK;
+  const int* row = g.table + (long long)b * g.table_stride;
+  auto block_at = [&](int i) QTTS_PG_INLINE { const int t = t0 + DW * i; return t < bl.ns ? t : t + bl.skip; };
+  // pages of 32 of the wave's blocks, one 16-key piece a lane (-1: none)
+  auto pages_from = [&](int i0) QTTS_PG_INLINE {
+    const int key = block_at(i0 + (lane >> 1)) * DKB + 16 * (lane & 1);
+    int p = -1;
+    if (i0 + (lane >> 1) < nt && key < len) p = *gmem(row + (key >> g.pages.shift));
+    return (unsigned)p < (unsigned)g.pages.num_pages ? p : -1;
+  };
+  int held = pages_from(0), next_held = 0;
+  uint64_t has = __builtin_amdgcn_ballot_w64(held >= 0);      // of block i: bits 2 (i & 31), + 1
+  auto issue = [&](int i) QTTS_PG_INLINE {
+    const int kb = block_at(i);
+    char* dst = buf + (i & 1) * 2 * BLK;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int page = __builtin_amdgcn_readlane(held, 2 * (i & 31) + u);
+      copy_piece<D>(g.pages, max(page, 0), kb * DKB + 16 * u, kvh, dst + u * 16 * D * 2, dst + BLK + u * 16 * D * 2, lane,
+                    [&](int key) QTTS_PG_INLINE { return (page >= 0) & (key < len) & ((key >= lo) | (key < g.sinks)); });
+    }
+  };
+
+  const float SL = g.scale_log2;
+  float m = -INFINITY, l = 0.0f;
+  f32x4 o[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) o[mb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  // transpose reads of V: row 4 gr + (c >> 2), chunk 2 mb + ((c & 3) >> 1), 8 bytes at 8 (c & 1)
+  const int vrow = 4 * gr + (c >> 2);
+  uint32_t vaddr[4];
+#pragma unroll
+  for (int mb = 0; mb < 4; ++mb)
+    vaddr[mb] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)buf + BLK + vrow * D * 2 +
+                ((2 * mb + ((c & 3) >> 1)) ^ (vrow & 7)) * 16 + 8 * (c & 1);
+
+  if (nt > 0) issue(0);
+#pragma unroll 1
+  for (int i = 0; i < nt; ++i) {
+    const uint64_t has_i = has >> (2 * (i & 31));
+    if (i + 1 < nt) {
+      if (((i + 1) & 31) == 0) {
+        held = pages_from(i + 1);
+        has = __builtin_amdgcn_ballot_w64(held >= 0);
+      }
+      issue(i + 1);
+      wait_vm_lds<NL>();
+    } else {
+      wait_vm_lds<0>();
+    }
+    asm volatile("" ::: "memory");
+    const char* K = buf + (i & 1) * 2 * BLK;
+    f32x4 sc[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      sc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const u32x4 k = *reinterpret_cast<const u32x4*>(K + (16 * u + c) * D * 2 + ((4 * s + gr) ^ (c & 7)) * 16);
+        sc[u] = E::mma16(k, q[s], sc[u]);
+      }
+    }
+    const int key0 = block_at(i) * DKB;
+    if (!((has_i & 3) == 3 && key0 + DKB <= len && (key0 >= lo || key0 + DKB <= g.sinks))) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = key0 + 16 * u + 4 * gr + r;
+          const bool seen = (((has_i >> u) & 1) != 0) & (key < len) & ((key >= lo) | (key < g.sinks));
+          sc[u][r] = seen ? sc[u][r] : -INFINITY;
+        }
+    }
+    float bm = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                     fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+    bm = fmaxf(bm, xlane_f<4>(bm));
+    bm = fmaxf(bm, xlane_f<5>(bm));
+    if (__builtin_amdgcn_ballot_w64(bm > m) != 0ull) {
+      const float mn = fmaxf(m, bm);
+      const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * SL);
+      l *= al;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[mb][r] *= al;
+      m = mn;
+    }
+    const float nm = m == -INFINITY ? 0.0f : -m * SL;
+    u32x4 ph, pl;
+    float sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[u][2 * h], SL, nm)), e1 = __builtin_amdgcn_exp2f(fmaf(sc[u][2 * h + 1], SL, nm));
+        sum += e0 + e1;
+        const uint32_t p = E::pack(e0, e1);
+        ph[2 * u + h] = p;
+        pl[2 * u + h] = E::pack(e0 - E::lo(p), e1 - E::hi(p));
+      }
+    l += sum;
+    uint32_t va[4];
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb) va[mb] = vaddr[mb] + (i & 1) * 2 * BLK;
+    auto pv = [&](int half, const u32x2 (&a)[4], const u32x2 (&bq)[4]) QTTS_PG_INLINE {
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb) {
+        const u32x4 v = {a[mb][0], a[mb][1], bq[mb][0], bq[mb][1]};
+        o[4 * half + mb] = E::mma16(v, ph, o[4 * half + mb]);
+        o[4 * half + mb] = E::mma16(v, pl, o[4 * half + mb]);
+      }
+    };
+    u32x2 a[4], bq[4];
+    tr_read8<0, 16 * D * 2>(va, a, bq);
+    pv(0, a, bq);
+    if constexpr (D == 128) {
+      tr_read8<128, 16 * D * 2>(va, a, bq);
+      pv(1, a, bq);
+    }
+  }
+  l += xlane_f<4>(l);
+  l += xlane_f<5>(l);
+
+  // join the waves: M = max m_w, L = sum l_w e^(m_w - M), O = sum O_w e^(m_w - M)
+  __syncthreads();                               // every buffer is dead
+  float* sml = reinterpret_cast<float*>(smem + DW * D * 16 * 4);
+  if (gr == 0) {
+    sml[(2 * w) * 16 + c] = m;
+    sml[(2 * w + 1) * 16 + c] = l;
+  }
+  __syncthreads();
+  float M = -INFINITY, L = 0.0f;
+#pragma unroll
+  for (int v = 0; v < DW; ++v) M = fmaxf(M, sml[2 * v * 16 + c]);
+#pragma unroll
+  for (int v = 0; v < DW; ++v) {
+    const float mv = sml[2 * v * 16 + c];
+    L += mv == -INFINITY ? sml[(2 * v + 1) * 16 + c] : sml[(2 * v + 1) * 16 + c] * __builtin_amdgcn_exp2f((mv - M) * SL);
+  }
+  const float sw = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - M) * SL);
+  float* so = reinterpret_cast<float*>(smem);    // [wave][head][channel]
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    f32x4 x;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = o[mb][r] * sw;
+    *reinterpret_cast<f32x4*>(so + (w * 16 + c) * D + 16 * mb + 4 * gr) = x;
+  }
+  if (w == 0 && gr == 0) {
+    sml[DW * 2 * 16 + c] = M;
+    sml[DW * 2 * 16 + 16 + c] = L;
+  }
+  __syncthreads();
+  const bool whole = units == 1;
+  for (int e = threadIdx.x; e < nh * D / 4; e += 64 * DW) {
+    const int h = e / (D / 4), d = 4 * (e % (D / 4));
+    f32x4 x = *reinterpret_cast<const f32x4*>(so + h * D + d);
+#pragma unroll
+    for (int v = 1; v < DW; ++v) x += *reinterpret_cast<const f32x4*>(so + (v * 16 + h) * D + d);
+    if (whole) {
+      const float Lh = sml[DW * 2 * 16 + 16 + h];
+      const float rl = Lh == 0.0f ? 0.0f : 1.0f / Lh;
+      u32x2 p;
+      p[0] = E::pack(x[0] * rl, x[1] * rl);
+      p[1] = E::pack(x[2] * rl, x[3] * rl);
+      *reinterpret_cast<u32x2*>(g.out + (long long)b * g.o_token + (long long)(head0 + h) * g.o_head + d) = p;
+    } else {
+      const long long at = ((long long)b * g.hq + head0 + h) * g.splits + unit;
+      *reinterpret_cast<f32x4*>(g.part + at * D + d) = x;
+      if (d == 0) {
+        g.part_ml[2 * at] = sml[DW * 2 * 16 + h];
+        g.part_ml[2 * at + 1] = sml[DW * 2 * 16 + 16 + h];
+      }
+    }
+  }
+}
+
+// The units of a request's head joined in key order: one wave per (request, query head).
+template <class E, int D>
+__global__ void __launch_bounds__(256) decode_join_kernel(const AttnArgs g) {
+  constexpr int DL = D / 64;
+  const int lane = threadIdx.x & 63;
+  const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= (long long)g.requests * g.hq) return;
+  const int b = (int)(id / g.hq), h = (int)(id % g.hq);
+  const int len = request_len(g, b);
+  const Blocks bl = blocks_of<DKB>(g.window > 0 ? max(len - g.window, 0) : 0, len, g.sinks);
+  const int per = max(g.blocks, (bl.n + g.splits - 1) / g.splits), units = (bl.n + per - 1) / per;
+  if (units <= 1) return;
+  const float* ml = g.part_ml + 2 * id * g.splits;
+  const float* po = g.part + id * g.splits * D + DL * lane;
+  float M = -INFINITY;
+  for (int u = lane; u < units; u += 64) M = fmaxf(M, ml[2 * u]);
+  M = group_max<64>(M);
+  float L = 0.0f, x[DL] = {};
+#pragma unroll 4
+  for (int u = 0; u < units; ++u) {
+    const float mu = ml[2 * u], wu = mu == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((mu - M) * g.scale_log2);
+    L += ml[2 * u + 1] * wu;
+#pragma unroll
+    for (int i = 0; i < DL; ++i) x[i] += po[(long long)u * D + i] * wu;
+  }
+  const float rl = L == 0.0f ? 0.0f : 1.0f / L;
+  uint16_t* op = g.out + (long long)b * g.o_token + (long long)h * g.o_head + DL * lane;
+  if constexpr (DL == 2) {
+    *reinterpret_cast<uint32_t*>(op) = E::pack(x[0] * rl, x[1] * rl);
+  } else {
+    *op = (uint16_t)E::pack(x[0] * rl, 0.0f);
+  }
+}
+
+// ---- prefill -------------------------------------------------------------------------------
+// The query rows of a request and KV head are its tokens times the group's heads, row r = token r / group,
+// head r % group, so that any group size fills the tiles. One workgroup of 4 waves takes PM = 128 rows, wave
+// w rows 32 w .. , and walks the 64-key blocks that any of them sees; K and V of a block come by DMA into
+// one of two LDS buffers, one block ahead, and the 4 waves share them. Bound by the matrix units, the LDS
+// reads that feed them and the exponentials, about equally: a 32 x 64 block of a wave is 32 MFMAs (1,024
+// cycles), 32 KB of LDS reads and 32 exponentials a lane, and the two workgroups of a CU fill each other's
+// waits.
+//   S^T = K Q^T on MFMA 32x32x16 (A: 32 keys from LDS, B: the rows in registers): lane (hf, c) holds row c's
+//     scores of keys 8 (r >> 2) + 4 hf + (r & 3), so a row's max and sum are in-lane and one exchange.
+//   O^T += V^T P^T with the score registers as P^T (k-index 8 hf + j of step kk is key 16 kk + 8 (j >> 2) +
+//     4 hf + (j & 3)) and V^T by LDS transpose reads. P is rounded to the element type, as V is; its sum
+//     is of the unrounded values in f32.
+// The running max moves only when a row's block max passes it by more than a factor 2^8 of the weights.
+// A weight that is masked is 0, but 0 times an infinite or NaN v_j is NaN, and a key may be hidden from one
+// row of a tile and seen by another: rows that end with a number that is not finite are summed again over
+// the keys that they see, one by one (exact_rows).
+constexpr int PWV = 4;
+constexpr int PM = 32 * PWV;          // rows of a tile
+constexpr int PKB = 64;               // keys of a block
+
+// Row `r` of (request b, KV head kvh) again, key by key: the wave's lanes take D / 64 channels each.
+template <class E, int D>
+__device__ __forceinline__ void exact_row(const AttnArgs& g, int b, int kvh, int token, int head, int pos) {
+  constexpr int DL = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int* row = g.table + (long long)b * g.table_stride;
+  auto at2 = [&](const uint16_t* p) QTTS_PG_INLINE {
+    float2 f;
+    if constexpr (DL == 2) {
+      const uint32_t v = *gmem(reinterpret_cast<const uint32_t*>(p + 2 * lane));
+      f.x = E::lo(v);
+      f.y = E::hi(v);
+    } else {
+      f.x = E::lo((uint32_t)*gmem(p + lane));
+      f.y = 0.0f;
+    }
+    return f;
+  };
+  const float2 q = at2(g.q + (long long)token * g.q_token + (long long)head * g.q_head);
+  const int lo = g.window > 0 ? max(pos - g.window + 1, 0) : 0;
+  float m = -INFINITY, l = 0.0f, x = 0.0f, y = 0.0f;
+  for (int key = 0; key <= pos; ++key) {
+    if (key < lo && key >= g.sinks) {
+      key = lo - 1;
+      continue;
+    }
+    const int page = *gmem(row + (key >> g.pages.shift));
+    if ((unsigned)page >= (unsigned)g.pages.num_pages) continue;
+    const long long at = (long long)page * g.pages.page_stride + (long long)kvh * g.pages.head_stride +
+                         (long long)(key & ((1 << g.pages.shift) - 1)) * g.pages.slot_stride;
+    const float2 k = at2(g.pages.k + at), v = at2(g.pages.v + at);
+    const float s = group_sum<64>(q.x * k.x + q.y * k.y);
+    if (s == -INFINITY) continue;
+    const float mn = fmaxf(m, s);
+    const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * g.scale_log2);
+    const float e = __builtin_amdgcn_exp2f((s - mn) * g.scale_log2);
+    l = (m == -INFINITY ? l : l * al) + e;       // (m is -inf still after a NaN score: keep it)
+    x = (m == -INFINITY ? x : x * al) + e * v.x;
+    y = (m == -INFINITY ? y : y * al) + e * v.y;
+    m = mn;
+  }
+  const float rl = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* op = g.out + (long long)token * g.o_token + (long long)head * g.o_head + DL * lane;
+  if constexpr (DL == 2) *reinterpret_cast<uint32_t*>(op) = E::pack(x * rl, y * rl);
+  else *op = (uint16_t)E::pack(x * rl, 0.0f);
+}
+
+// The tile-th tile of PM rows over all requests: its request and its place in it; request -1 past the end.
+// Every lane takes a request, 64 at a time. Tiles are counted from the last back (the longest keys first).
+struct TilePlace {
+  int b, tile, first, n;              // request, tile in it, first token, tokens
+};
+__device__ __forceinline__ int tiles_of(const AttnArgs& g, int b, int* first, int* n) {
+  int f = 0, k = 0;
+  if (b < g.requests) {
+    f = min(max(g.cu[b], 0), g.tokens);
+    k = max(min(max(g.cu[b + 1], 0), g.tokens) - f, 0);
+  }
+  *first = f;
+  *n = k;
+  return (int)(((long long)k * g.group + PM - 1) / PM);
+}
+__device__ __forceinline__ TilePlace find_tile(const AttnArgs& g, int back) {
+  const int lane = threadIdx.x & 63;
+  for (int b0 = (g.requests - 1) & ~63; b0 >= 0; b0 -= 64) {
+    int first, n;
+    const int own = tiles_of(g, b0 + lane, &first, &n);
+    int after = own;                  // tiles of the lane's request and those behind it
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_down(after, o, 64);
+      if (lane + o < 64) after += y;
+    }
+    const int all = __builtin_amdgcn_readfirstlane(after);
+    if (back < all) {
+      const int src = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(after > back));   // the last such lane
+      TilePlace p;
+      p.b = b0 + src;
+      p.tile = __builtin_amdgcn_readlane(after, src) - 1 - back;   // those of later requests come first
+      p.first = __builtin_amdgcn_readlane(first, src);
+      p.n = __builtin_amdgcn_readlane(n, src);
+      return p;
+    }
+    back -= all;
+  }
+  return TilePlace{-1, 0, 0, 0};
+}
+
+template <class E, int D>
+__global__ void __launch_bounds__(64 * PWV, 2) prefill_kernel(const AttnArgs g) {
+  constexpr int BLK = PKB * D * 2;
+  constexpr int MB = D / 32, KS = D / 16;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * BLK];   // (K, V) x 2 buffers
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int hf = lane >> 5, c = lane & 31;
+  const int kvh = blockIdx.x % g.hkv;
+  const TilePlace at = find_tile(g, blockIdx.x / g.hkv);
+  if (at.b < 0) return;
+  const int len = request_len(g, at.b), p0 = len - at.n;   // (p0 < 0: more tokens than keys; those before key 0 see none)
+  const int rows = at.n * g.group;                          // (the host bounds tokens * group)
+  const int r0 = at.tile * PM, i0 = r0 / g.group, i1 = (min(r0 + PM, rows) - 1) / g.group;
+  const int end = max(p0 + i1 + 1, 0);                      // keys that the tile's last token sees
+  const int lo = g.window > 0 ? max(p0 + i0 + 1 - g.window, 0) : 0;
+  const Blocks bl = blocks_of<PKB>(lo, end, g.sinks);
+
+  // this lane's row, and the first and last position of the wave's
+  const int r = min(r0 + 32 * w + c, rows - 1), ti = r / g.group, head = kvh * g.group + (r - ti * g.group);
+  const bool stored = r0 + 32 * w + c < rows;
+  const int pos = p0 + ti;
+  const int wlo = p0 + min(r0 + 32 * w, rows - 1) / g.group, whi = p0 + min(r0 + 32 * w + 31, rows - 1) / g.group;
+  const int first_key = g.window > 0 ? pos - g.window + 1 : 0;   // of the row's window
+
+  u32x4 q[KS];
+  const uint16_t* qp = g.q + (long long)(at.first + ti) * g.q_token + (long long)head * g.q_head + 8 * hf;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) q[s] = ldw(qp + 16 * s);
+
+  const int* row = g.table + (long long)at.b * g.table_stride;
+  auto block_at = [&](int i) QTTS_PG_INLINE { return i < bl.ns ? i : i + bl.skip; };
+  // pages of 16 blocks, one 16-key piece a lane (-1: none)
+  auto pages_from = [&](int b0) QTTS_PG_INLINE {
+    const int key = block_at(b0 + (lane >> 2)) * PKB + 16 * (lane & 3);
+    int p = -1;
+    if (b0 + (lane >> 2) < bl.n && key < end) p = *gmem(row + (key >> g.pages.shift));
+    return (unsigned)p < (unsigned)g.pages.num_pages ? p : -1;
+  };
+  int held = pages_from(0);
+  uint64_t has = __builtin_amdgcn_ballot_w64(held >= 0);
+  auto issue = [&](int i) QTTS_PG_INLINE {                   // wave w copies piece w of the block
+    const int page = __builtin_amdgcn_readlane(held, 4 * (i & 15) + w);
+    char* dst = smem + (i & 1) * 2 * BLK + w * 16 * D * 2;
+    copy_piece<D>(g.pages, max(page, 0), block_at(i) * PKB + 16 * w, kvh, dst, dst + BLK, lane,
+                  [&](int key) QTTS_PG_INLINE { return (page >= 0) & (key < end) & ((key >= lo) | (key < g.sinks)); });
+  };
+
+  const float SL = g.scale_log2;
+  float m = -INFINITY, l = 0.0f;
+  f32x16 o[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[mb][e] = 0.0f;
+  const int gi = lane & 15, gg = lane >> 4;
+  const int vrow = 4 * (gg >> 1) + (gi >> 2), vch = 2 * (gg & 1) + ((gi & 3) >> 1);
+  uint32_t vaddr[4];
+#pragma unroll
+  for (int mb = 0; mb < 4; ++mb)
+    vaddr[mb] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + BLK + vrow * D * 2 +
+                ((4 * (mb % MB) + vch) ^ (vrow & 7)) * 16 + 8 * (gi & 1);
+
+  if (bl.n > 0) issue(0);
+#pragma unroll 1
+  for (int i = 0; i < bl.n; ++i) {
+    wait_vm_lds<0>();                 // this wave's copies have landed, its reads of the other buffer are done
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const int has_i = (int)(has >> (4 * (i & 15))) & 15;
+    if (i + 1 < bl.n) {
+      if (((i + 1) & 15) == 0) {
+        held = pages_from(i + 1);
+        has = __builtin_amdgcn_ballot_w64(held >= 0);
+      }
+      issue(i + 1);
+    }
+    const int key0 = block_at(i) * PKB;
+    // blocks that no row of the wave sees
+    if (key0 > whi || (g.window > 0 && key0 >= g.sinks && key0 + PKB <= wlo - g.window + 1)) continue;
+    const char* K = smem + (i & 1) * 2 * BLK;
+    float sc[32];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      f32x16 a;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) a[e] = 0.0f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+        a = E::mma32(*reinterpret_cast<const u32x4*>(K + (32 * u + c) * D * 2 + ((2 * s + hf) ^ (c & 7)) * 16), q[s], a);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[16 * u + e] = a[e];
+    }
+    const bool all = has_i == 15 && key0 + PKB - 1 <= wlo && (g.window == 0 || key0 > whi - g.window || key0 + PKB <= g.sinks);
+    if (!all) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int in = 32 * u + 8 * (e >> 2) + 4 * hf + (e & 3), key = key0 + in;
+          const bool seen = (((has_i >> (in >> 4)) & 1) != 0) & (key <= pos) & ((key >= first_key) | (key < g.sinks));
+          sc[16 * u + e] = seen ? sc[16 * u + e] : -INFINITY;
+        }
+    }
+    float bm = sc[0];
+#pragma unroll
+    for (int e = 1; e < 32; ++e) bm = fmaxf(bm, sc[e]);
+    bm = fmaxf(bm, xlane_f<5>(bm));
+    if (__builtin_amdgcn_ballot_w64(bm > m + 8.0f / SL) != 0ull) {
+      const float mn = fmaxf(m, bm);
+      const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * SL);
+      l *= al;
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[mb][e] *= al;
+      m = mn;
+    }
+    const float nm = m == -INFINITY ? 0.0f : -m * SL;
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], SL, nm));
+      sum += sc[e];
+    }
+    l += sum;
+    uint32_t va[4];
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb) va[mb] = vaddr[mb] + (i & 1) * 2 * BLK;
+    auto pv = [&](auto kk_) QTTS_PG_INLINE {
+      constexpr int kk = decltype(kk_)::value;
+      u32x4 p;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = E::pack(sc[8 * kk + 2 * j], sc[8 * kk + 2 * j + 1]);
+      u32x2 a[4], bq[4];
+      if constexpr (D == 128) {
+        tr_read8<16 * kk * D * 2, 8 * D * 2>(va, a, bq);
+      } else {
+        tr_read4<16 * kk * D * 2, 8 * D * 2>(va, a, bq);
+      }
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        const u32x4 v = {a[mb][0], a[mb][1], bq[mb][0], bq[mb][1]};
+        o[mb] = E::mma32(v, p, o[mb]);
+      }
+    };
+    pv(std::integral_constant<int, 0>{});
+    pv(std::integral_constant<int, 1>{});
+    pv(std::integral_constant<int, 2>{});
+    pv(std::integral_constant<int, 3>{});
+  }
+  l += xlane_f<5>(l);
+
+  // O^T: column = row c, register e of block mb = channel 32 mb + 8 (e >> 2) + 4 hf + (e & 3)
+  const float rl = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* op = g.out + (long long)(at.first + ti) * g.o_token + (long long)head * g.o_head + 4 * hf;
+  float worst = 0.0f;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      o[mb][e] *= rl;
+      worst += o[mb][e] - o[mb][e];   // NaN when one is not finite
+    }
+  worst += xlane_f<5>(worst);
+  uint64_t again = __builtin_amdgcn_ballot_w64(stored && !(worst == 0.0f)) & 0xffffffffull;
+  if (stored && worst == 0.0f) {
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        u32x2 p;
+        p[0] = E::pack(o[mb][4 * e], o[mb][4 * e + 1]);
+        p[1] = E::pack(o[mb][4 * e + 2], o[mb][4 * e + 3]);
+        *reinterpret_cast<u32x2*>(op + 32 * mb + 8 * e) = p;
+      }
+  }
+  while (again != 0ull) {
+    const int src = __builtin_ctzll(again);
+    again &= again - 1;
+    exact_row<E, D>(g, at.b, kvh, at.first + __builtin_amdgcn_readlane(ti, src), __builtin_amdgcn_readlane(head, src),
+                    __builtin_amdgcn_readlane(pos, src));
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------
+
+bool attn_ok(const QttsPagedCache* cache, int n_tokens, int hq, const void* q, long long q_token, long long q_head, const void* out,
+             long long o_token, long long o_head, const int* table, int width, long long table_stride, const int* lens,
+             int requests, float scale, int window, int sinks) {
+  if (!cache_ok(cache) || requests < 1 || n_tokens < 0 || hq < 1 || hq % cache->num_kv_heads != 0) return false;
+  if (q == nullptr || out == nullptr || table == nullptr || lens == nullptr) return false;
+  if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) != 0) return false;
+  if (((q_token | q_head | o_token | o_head) & 7) != 0) return false;
+  if (width < 1 || table_stride < width || (long long)width * cache->page_size > INT_MAX - 4096) return false;
+  if (!(scale > 0.0f) || !std::isfinite(scale) || window < 0 || sinks < 0) return false;
+  return (long long)n_tokens * hq <= INT_MAX / 2;
+}
+
+AttnArgs attn_args(const QttsPagedCache* cache, int hq, const void* q, long long q_token, long long q_head, void* out,
+                   long long o_token, long long o_head, const int* table, int width, long long table_stride,
+                   const int* lens, int requests, float scale, int window, int sinks) {
+  AttnArgs g{};
+  g.q = static_cast<const uint16_t*>(q);
+  g.out = static_cast<uint16_t*>(out);
+  g.q_token = q_token; g.q_head = q_head; g.o_token = o_token; g.o_head = o_head;
+  g.pages = pages_of(cache);
+  g.table = table;
+  g.table_stride = table_stride;
+  g.width = width;
+  g.lens = lens;
+  g.requests = requests;
+  g.hq = hq;
+  g.group = hq / cache->num_kv_heads;
+  g.hkv = cache->num_kv_heads;
+  g.scale_log2 = scale * 1.4426950408889634f;
+  g.window = window;
+  g.sinks = window > 0 ? sinks : 0;
+  return g;
+}
+
+// How decode splits a request: units of at least 4 blocks (one a wave), as many as give every CU work.
+struct Split {
+  int splits, blocks;
+};
+Split decode_split(int requests, int hkv, int group, int width, int page_size, int max_len, int window, int sinks) {
+  long long keys = std::min<long long>((long long)width * page_size, max_len);
+  if (window > 0) keys = std::min<long long>(keys, (long long)window + std::min<long long>(sinks, keys) + 2 * DKB);
+  const long long blocks = std::max<long long>(1, (keys + DKB - 1) / DKB);
+  const long long pairs = (long long)requests * hkv * ((group + 15) / 16);
+  const long long want = std::max<long long>(1, 1024 / pairs);
+  long long per = std::max<long long>(16, (blocks + want - 1) / want);
+  per = (per + DW - 1) / DW * DW;
+  const long long splits = (blocks + per - 1) / per;
+  return Split{(int)splits, (int)per};
+}
+
+template <class E, int D>
+void launch_decode(const AttnArgs& g, hipStream_t st) {
+  const int tiles = (g.group + 15) / 16;
+  hipLaunchKernelGGL((decode_kernel<E, D>), dim3((unsigned)((long long)g.requests * g.hkv * tiles * g.splits)), dim3(64 * DW), 0, st, g);
+  if (g.splits > 1)
+    hipLaunchKernelGGL((decode_join_kernel<E, D>), dim3((unsigned)(((long long)g.requests * g.hq + 3) / 4)), dim3(256), 0, st, g);
+}
+
+}  // namespace pg
+}  // namespace qtts
+
+using namespace qtts;
+using namespace qtts::pg;
+
+extern "C" {
+
+size_t qtts_paged_decode_workspace_bytes(int n_requests, int num_q_heads, int num_kv_heads, int head_dim, int table_width,
+                                         int page_size, int max_len, int window, int sinks) {
+  if (n_requests < 1 || num_kv_heads < 1 || num_q_heads < 1 || num_q_heads % num_kv_heads != 0 || head_dim < 1 ||
+      table_width < 1 || page_size < 1 || max_len < 1 || window < 0 || sinks < 0)
+    return 0;
+  const Split s = decode_split(n_requests, num_kv_heads, num_q_heads / num_kv_heads, table_width, page_size, max_len, window, sinks);
+  return s.splits == 1 ? 0 : (size_t)n_requests * num_q_heads * s.splits * (head_dim + 2) * 4;
+}
+
+hipError_t qtts_paged_attention_decode(const QttsPagedCache* cache, int n_requests, int num_q_heads, const void* q,
+                                       long long q_token_stride, long long q_head_stride, void* out,
+                                       long long out_token_stride, long long out_head_stride, const int* block_table,
+                                       int table_width, long long table_stride, const int* kv_lens, int max_len,
+                                       float scale, int window, int sinks, void* workspace, size_t workspace_bytes,
+                                       hipStream_t stream) {
+  if (!attn_ok(cache, n_requests, num_q_heads, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
+               block_table, table_width, table_stride, kv_lens, n_requests, scale, window, sinks) || max_len < 1)
+    return hipErrorInvalidValue;
+  AttnArgs g = attn_args(cache, num_q_heads, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
+                         block_table, table_width, table_stride, kv_lens, n_requests, scale, window, sinks);
+  const Split s = decode_split(n_requests, g.hkv, g.group, table_width, cache->page_size, max_len, window, sinks);
+  g.splits = s.splits;
+  g.blocks = s.blocks;
+  if (s.splits > 1) {
+    const size_t sums = (size_t)n_requests * num_q_heads * s.splits * cache->head_dim * 4;
+    const size_t need = qtts_paged_decode_workspace_bytes(n_requests, num_q_heads, g.hkv, cache->head_dim, table_width,
+                                                          cache->page_size, max_len, window, sinks);
+    if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
+      return hipErrorInvalidValue;
+    g.part = static_cast<float*>(workspace);
+    g.part_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + sums);
+  }
+  if ((long long)n_requests * g.hkv * ((g.group + 15) / 16) * g.splits > INT_MAX) return hipErrorInvalidValue;
+  if (cache->dtype == QTTS_BF16) {
+    if (cache->head_dim == 128) launch_decode<Bf16, 128>(g, stream);
+    else launch_decode<Bf16, 64>(g, stream);
+  } else {
+    if (cache->head_dim == 128) launch_decode<F16, 128>(g, stream);
+    else launch_decode<F16, 64>(g, stream);
+  }
+  return hipGetLastError();
+}
+
+hipError_t qtts_paged_attention_prefill(const QttsPagedCache* cache, int n_requests, int n_tokens, int num_q_heads,
+                                        const void* q, long long q_token_stride, long long q_head_stride, void* out,
+                                        long long out_token_stride, long long out_head_stride, const int* block_table,
+                                        int table_width, long long table_stride, const int* kv_lens, const int* cu_tokens,
+                                        float scale, int window, int sinks, hipStream_t stream) {
+  if (!attn_ok(cache, n_tokens, num_q_heads, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
+               block_table, table_width, table_stride, kv_lens, n_requests, scale, window, sinks) || cu_tokens == nullptr)
+    return hipErrorInvalidValue;
+  if (n_tokens == 0) return hipSuccess;
+  AttnArgs g = attn_args(cache, num_q_heads, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
+                         block_table, table_width, table_stride, kv_lens, n_requests, scale, window, sinks);
+  g.cu = cu_tokens;
+  g.tokens = n_tokens;
+  // every request ends with a tile that may be part empty; no more tiles than rows
+  const long long tiles = std::min((long long)n_tokens * g.group / PM + n_requests, (long long)n_tokens * g.group);
+  if (tiles * g.hkv > INT_MAX) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)(tiles * g.hkv)), block(64 * PWV);
+  if (cache->dtype == QTTS_BF16) {
+    if (cache->head_dim == 128) hipLaunchKernelGGL((prefill_kernel<Bf16, 128>), grid, block, 0, stream, g);
+    else hipLaunchKernelGGL((prefill_kernel<Bf16, 64>), grid, block, 0, stream, g);
+  } else {
+    if (cache->head_dim == 128) hipLaunchKernelGGL((prefill_kernel<F16, 128>), grid, block, 0, stream, g);
+    else hipLaunchKernelGGL((prefill_kernel<F16, 64>), grid, block, 0, stream, g);
+  }
+  return hipGetLastError();
+}
+
+}  // extern "C"
