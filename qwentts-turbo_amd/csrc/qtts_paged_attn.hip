@@ -62,8 +62,17 @@ __device__ __forceinline__ Blocks blocks_of(int lo, int end, int sinks) {
   return r;
 }
 
-// One 16-key piece of K and V into LDS by DMA, row r at r * 2 D bytes with its 16-byte chunk c at position
-// c ^ (r & 7). The descriptors begin at the piece's first row and end with its last, and rows that are
+// Staged rows: row r of a block at r * 2 D bytes, its 16-byte chunk c at position c ^ swz(r). LDS serves 256 bytes
+// a cycle from 64 banks; with this permutation the 16 rows of an operand read (one chunk each) and the 4 rows x
+// 64 bytes of a transpose read fall on different banks (with c ^ (r & 7) the transpose reads of 4 rows fell on the
+// same 64 bytes: two thirds of the LDS cycles were conflicts).
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  if constexpr (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else return ((r << 1) & 4) | ((r >> 1) & 2) | ((r >> 3) & 1);
+}
+
+// One 16-key piece of K and V into LDS by DMA. The descriptors begin at the piece's first row and end with its last, and rows that are
 // not `seen` are asked for past the end: they come as zeros.
 template <int D, class Seen>
 __device__ __forceinline__ void copy_piece(const Pages& pg, int page, int key0, int kvh, char* k_dst, char* v_dst, int lane,
@@ -77,7 +86,7 @@ __device__ __forceinline__ void copy_piece(const Pages& pg, int page, int key0, 
 #pragma unroll
   for (int i = 0; i < 16 / RPI; ++i) {
     const int r = RPI * i + lane / CPR;
-    const int in = r * pg.slot_stride * 2 + ((lane % CPR) ^ (r & 7)) * 16;
+    const int in = r * pg.slot_stride * 2 + ((lane % CPR) ^ swz<D>(r)) * 16;
     const int off = seen(key0 + r) ? in : 0x7fffff00;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lvoid_t*)(k_dst + i * 1024), 16, off, 0, 0, 0);
     __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lvoid_t*)(v_dst + i * 1024), 16, off, 0, 0, 0);
@@ -101,30 +110,29 @@ __device__ __forceinline__ void copy_piece(const Pages& pg, int page, int key0, 
 constexpr int DW = 4;                 // waves
 constexpr int DKB = 32;               // keys of a block
 
-// The transpose reads of an MFMA step: 4 keys at LDS addresses a[0..3] + OFF and 4 more T bytes further, of
-// each channel block. In assembly with their wait: before the builtin the compiler waits for every DMA in
-// flight, the next block's among them.
-template <int OFF, int T>
-__device__ __forceinline__ void tr_read8(const uint32_t (&a)[4], u32x2 (&lo)[4], u32x2 (&hi)[4]) {
+// The transpose reads of an MFMA step: 4 keys at LDS addresses a[..] + A and 4 more at b[..] + B, of each channel
+// block. In assembly with their wait: before the builtin the compiler waits for every DMA in flight, the next
+// block's among them.
+template <int A, int B>
+__device__ __forceinline__ void tr_read8(const uint32_t (&a)[4], const uint32_t (&b)[4], u32x2 (&lo)[4], u32x2 (&hi)[4]) {
   asm volatile(
-      "ds_read_b64_tr_b16 %0, %8 offset:%c12\n\tds_read_b64_tr_b16 %4, %8 offset:%c13\n\t"
-      "ds_read_b64_tr_b16 %1, %9 offset:%c12\n\tds_read_b64_tr_b16 %5, %9 offset:%c13\n\t"
-      "ds_read_b64_tr_b16 %2, %10 offset:%c12\n\tds_read_b64_tr_b16 %6, %10 offset:%c13\n\t"
-      "ds_read_b64_tr_b16 %3, %11 offset:%c12\n\tds_read_b64_tr_b16 %7, %11 offset:%c13\n\t"
+      "ds_read_b64_tr_b16 %0, %8 offset:%c16\n\tds_read_b64_tr_b16 %4, %12 offset:%c17\n\t"
+      "ds_read_b64_tr_b16 %1, %9 offset:%c16\n\tds_read_b64_tr_b16 %5, %13 offset:%c17\n\t"
+      "ds_read_b64_tr_b16 %2, %10 offset:%c16\n\tds_read_b64_tr_b16 %6, %14 offset:%c17\n\t"
+      "ds_read_b64_tr_b16 %3, %11 offset:%c16\n\tds_read_b64_tr_b16 %7, %15 offset:%c17\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(lo[2]), "=&v"(lo[3]), "=&v"(hi[0]), "=&v"(hi[1]), "=&v"(hi[2]), "=&v"(hi[3])
-      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "i"(OFF), "i"(OFF + T)
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]), "i"(A), "i"(B)
       : "memory");
 }
-
-template <int OFF, int T>
-__device__ __forceinline__ void tr_read4(const uint32_t (&a)[4], u32x2 (&lo)[4], u32x2 (&hi)[4]) {
+template <int A, int B>
+__device__ __forceinline__ void tr_read4(const uint32_t (&a)[4], const uint32_t (&b)[4], u32x2 (&lo)[4], u32x2 (&hi)[4]) {
   asm volatile(
-      "ds_read_b64_tr_b16 %0, %4 offset:%c6\n\tds_read_b64_tr_b16 %2, %4 offset:%c7\n\t"
-      "ds_read_b64_tr_b16 %1, %5 offset:%c6\n\tds_read_b64_tr_b16 %3, %5 offset:%c7\n\t"
+      "ds_read_b64_tr_b16 %0, %4 offset:%c8\n\tds_read_b64_tr_b16 %2, %6 offset:%c9\n\t"
+      "ds_read_b64_tr_b16 %1, %5 offset:%c8\n\tds_read_b64_tr_b16 %3, %7 offset:%c9\n\t"
       "s_waitcnt lgkmcnt(0)"
       : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(hi[0]), "=&v"(hi[1])
-      : "v"(a[0]), "v"(a[1]), "i"(OFF), "i"(OFF + T)
+      : "v"(a[0]), "v"(a[1]), "v"(b[0]), "v"(b[1]), "i"(A), "i"(B)
       : "memory");
 }
 
@@ -192,7 +200,7 @@ __global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
 #pragma unroll
   for (int mb = 0; mb < 4; ++mb)
     vaddr[mb] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)buf + BLK + vrow * D * 2 +
-                ((2 * mb + ((c & 3) >> 1)) ^ (vrow & 7)) * 16 + 8 * (c & 1);
+                ((2 * mb + ((c & 3) >> 1)) ^ swz<D>(vrow)) * 16 + 8 * (c & 1);
 
   if (nt > 0) issue(0);
 #pragma unroll 1
@@ -216,7 +224,7 @@ __global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
       sc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const u32x4 k = *reinterpret_cast<const u32x4*>(K + (16 * u + c) * D * 2 + ((4 * s + gr) ^ (c & 7)) * 16);
+        const u32x4 k = *reinterpret_cast<const u32x4*>(K + (16 * u + c) * D * 2 + ((4 * s + gr) ^ swz<D>(c)) * 16);
         sc[u] = E::mma16(k, q[s], sc[u]);
       }
     }
@@ -271,10 +279,12 @@ __global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
       }
     };
     u32x2 a[4], bq[4];
-    tr_read8<0, 16 * D * 2>(va, a, bq);
+    tr_read8<0, 16 * D * 2>(va, va, a, bq);
     pv(0, a, bq);
     if constexpr (D == 128) {
-      tr_read8<128, 16 * D * 2>(va, a, bq);
+#pragma unroll
+      for (int mb = 0; mb < 4; ++mb) va[mb] ^= 128;   // channels 64 ..
+      tr_read8<0, 16 * D * 2>(va, va, a, bq);
       pv(1, a, bq);
     }
   }
@@ -371,24 +381,23 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const AttnArgs g) {
 
 // ---- prefill -------------------------------------------------------------------------------
 // The query rows of a request and KV head are its tokens times the group's heads, row r = token r / group,
-// head r % group, so that any group size fills the tiles. One workgroup of 4 waves takes PM = 128 rows, wave
-// w rows 32 w .. , and walks the 64-key blocks that any of them sees; K and V of a block come by DMA into
-// one of two LDS buffers, one block ahead, and the 4 waves share them. Bound by the matrix units, the LDS
-// reads that feed them and the exponentials, about equally: a 32 x 64 block of a wave is 32 MFMAs (1,024
-// cycles), 32 KB of LDS reads and 32 exponentials a lane, and the two workgroups of a CU fill each other's
-// waits.
+// head r % group, so that any group size fills the tiles. One workgroup of 8 waves takes a tile of 32 NR rows
+// and walks the keys that any of them sees 128 at a time: wave (ks, wr) takes rows 32 wr .. and the key
+// block ks of each step (NS blocks of 128 / NS keys, NR = 8 / NS). K and V of a step come by DMA, a 16-key piece
+// a wave, into one of two LDS buffers, one step ahead. The key splits halve (NS = 2) or quarter (NS = 4) the
+// chain of steps of a tile, which is what a causal launch waits for: its last tiles see all the keys.
 //   S^T = K Q^T on MFMA 32x32x16 (A: 32 keys from LDS, B: the rows in registers): lane (hf, c) holds row c's
 //     scores of keys 8 (r >> 2) + 4 hf + (r & 3), so a row's max and sum are in-lane and one exchange.
 //   O^T += V^T P^T with the score registers as P^T (k-index 8 hf + j of step kk is key 16 kk + 8 (j >> 2) +
 //     4 hf + (j & 3)) and V^T by LDS transpose reads. P is rounded to the element type, as V is; its sum
 //     is of the unrounded values in f32.
-// The running max moves only when a row's block max passes it by more than a factor 2^8 of the weights.
+// The running max moves only when a row's block max passes it by more than a factor 2^8 of the weights. The
+// splits of a row join through LDS in key order.
 // A weight that is masked is 0, but 0 times an infinite or NaN v_j is NaN, and a key may be hidden from one
 // row of a tile and seen by another: rows that end with a number that is not finite are summed again over
-// the keys that they see, one by one (exact_rows).
-constexpr int PWV = 4;
-constexpr int PM = 32 * PWV;          // rows of a tile
-constexpr int PKB = 64;               // keys of a block
+// the keys that they see, one by one (exact_row).
+constexpr int PWV = 8;                // waves
+constexpr int PSTEP = 128;            // keys of a step
 
 // Row `r` of (request b, KV head kvh) again, key by key: the wave's lanes take D / 64 channels each.
 template <class E, int D>
@@ -437,11 +446,12 @@ __device__ __forceinline__ void exact_row(const AttnArgs& g, int b, int kvh, int
   else *op = (uint16_t)E::pack(x * rl, 0.0f);
 }
 
-// The tile-th tile of PM rows over all requests: its request and its place in it; request -1 past the end.
-// Every lane takes a request, 64 at a time. Tiles are counted from the last back (the longest keys first).
+// A tile of PM rows over all requests, counted from the last back (the longest keys first): its request and its
+// place in it; request -1 past the first. Every lane takes a request, 64 at a time.
 struct TilePlace {
   int b, tile, first, n;              // request, tile in it, first token, tokens
 };
+template <int PM>
 __device__ __forceinline__ int tiles_of(const AttnArgs& g, int b, int* first, int* n) {
   int f = 0, k = 0;
   if (b < g.requests) {
@@ -452,11 +462,12 @@ __device__ __forceinline__ int tiles_of(const AttnArgs& g, int b, int* first, in
   *n = k;
   return (int)(((long long)k * g.group + PM - 1) / PM);
 }
+template <int PM>
 __device__ __forceinline__ TilePlace find_tile(const AttnArgs& g, int back) {
   const int lane = threadIdx.x & 63;
   for (int b0 = (g.requests - 1) & ~63; b0 >= 0; b0 -= 64) {
     int first, n;
-    const int own = tiles_of(g, b0 + lane, &first, &n);
+    const int own = tiles_of<PM>(g, b0 + lane, &first, &n);
     int after = own;                  // tiles of the lane's request and those behind it
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -478,28 +489,31 @@ __device__ __forceinline__ TilePlace find_tile(const AttnArgs& g, int back) {
   return TilePlace{-1, 0, 0, 0};
 }
 
-template <class E, int D>
-__global__ void __launch_bounds__(64 * PWV, 2) prefill_kernel(const AttnArgs g) {
-  constexpr int BLK = PKB * D * 2;
+template <class E, int D, int NS>
+__global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(const AttnArgs g) {
+  constexpr int NR = PWV / NS, PM = 32 * NR, KB = PSTEP / NS;   // rows of a tile, keys of a wave's block
+  constexpr int NU = KB / 32, PPB = KB / 16;                    // 32-key score blocks, pieces of a block
+  constexpr int BUF = PSTEP * D * 2;                            // bytes of a step's K or V
   constexpr int MB = D / 32, KS = D / 16;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * BLK];   // (K, V) x 2 buffers
+  __shared__ __attribute__((aligned(1024))) char smem[4 * BUF + PWV * 2 * 32 * 4];   // (K, V) x 2 buffers; (m, l) of the join
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int hf = lane >> 5, c = lane & 31;
+  const int hf = lane >> 5, c = lane & 31, wr = w % NR, ks = w / NR;
   const int kvh = blockIdx.x % g.hkv;
-  const TilePlace at = find_tile(g, blockIdx.x / g.hkv);
+  const TilePlace at = find_tile<PM>(g, blockIdx.x / g.hkv);
   if (at.b < 0) return;
   const int len = request_len(g, at.b), p0 = len - at.n;   // (p0 < 0: more tokens than keys; those before key 0 see none)
   const int rows = at.n * g.group;                          // (the host bounds tokens * group)
   const int r0 = at.tile * PM, i0 = r0 / g.group, i1 = (min(r0 + PM, rows) - 1) / g.group;
   const int end = max(p0 + i1 + 1, 0);                      // keys that the tile's last token sees
   const int lo = g.window > 0 ? max(p0 + i0 + 1 - g.window, 0) : 0;
-  const Blocks bl = blocks_of<PKB>(lo, end, g.sinks);
+  const Blocks bl = blocks_of<KB>(lo, end, g.sinks);
+  const int steps = (bl.n + NS - 1) / NS;
 
   // this lane's row, and the first and last position of the wave's
-  const int r = min(r0 + 32 * w + c, rows - 1), ti = r / g.group, head = kvh * g.group + (r - ti * g.group);
-  const bool stored = r0 + 32 * w + c < rows;
+  const int r = min(r0 + 32 * wr + c, rows - 1), ti = r / g.group, head = kvh * g.group + (r - ti * g.group);
+  const bool stored = r0 + 32 * wr + c < rows;
   const int pos = p0 + ti;
-  const int wlo = p0 + min(r0 + 32 * w, rows - 1) / g.group, whi = p0 + min(r0 + 32 * w + 31, rows - 1) / g.group;
+  const int wlo = p0 + min(r0 + 32 * wr, rows - 1) / g.group, whi = p0 + min(r0 + 32 * wr + 31, rows - 1) / g.group;
   const int first_key = g.window > 0 ? pos - g.window + 1 : 0;   // of the row's window
 
   u32x4 q[KS];
@@ -508,20 +522,20 @@ __global__ void __launch_bounds__(64 * PWV, 2) prefill_kernel(const AttnArgs g) 
   for (int s = 0; s < KS; ++s) q[s] = ldw(qp + 16 * s);
 
   const int* row = g.table + (long long)at.b * g.table_stride;
-  auto block_at = [&](int i) QTTS_PG_INLINE { return i < bl.ns ? i : i + bl.skip; };
-  // pages of 16 blocks, one 16-key piece a lane (-1: none)
-  auto pages_from = [&](int b0) QTTS_PG_INLINE {
-    const int key = block_at(b0 + (lane >> 2)) * PKB + 16 * (lane & 3);
+  auto key_of = [&](int t) QTTS_PG_INLINE { return (t < bl.ns ? t : t + bl.skip) * KB; };   // first key of block t
+  // pages of 8 steps, one 16-key piece a lane (-1: none)
+  auto pages_from = [&](int i0) QTTS_PG_INLINE {
+    const int t = (i0 + (lane >> 3)) * NS + (lane & 7) / PPB, key = key_of(t) + 16 * (lane & (PPB - 1));
     int p = -1;
-    if (b0 + (lane >> 2) < bl.n && key < end) p = *gmem(row + (key >> g.pages.shift));
+    if (t < bl.n && key < end) p = *gmem(row + (key >> g.pages.shift));
     return (unsigned)p < (unsigned)g.pages.num_pages ? p : -1;
   };
   int held = pages_from(0);
   uint64_t has = __builtin_amdgcn_ballot_w64(held >= 0);
-  auto issue = [&](int i) QTTS_PG_INLINE {                   // wave w copies piece w of the block
-    const int page = __builtin_amdgcn_readlane(held, 4 * (i & 15) + w);
-    char* dst = smem + (i & 1) * 2 * BLK + w * 16 * D * 2;
-    copy_piece<D>(g.pages, max(page, 0), block_at(i) * PKB + 16 * w, kvh, dst, dst + BLK, lane,
+  auto issue = [&](int i) QTTS_PG_INLINE {                   // wave w copies piece w of the step
+    const int page = __builtin_amdgcn_readlane(held, 8 * (i & 7) + w);
+    char* dst = smem + (i & 1) * 2 * BUF + w * 16 * D * 2;
+    copy_piece<D>(g.pages, max(page, 0), key_of(i * NS + w / PPB) + 16 * (w % PPB), kvh, dst, dst + BUF, lane,
                   [&](int key) QTTS_PG_INLINE { return (page >= 0) & (key < end) & ((key >= lo) | (key < g.sinks)); });
   };
 
@@ -532,58 +546,58 @@ __global__ void __launch_bounds__(64 * PWV, 2) prefill_kernel(const AttnArgs g) 
   for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[mb][e] = 0.0f;
+  // transpose reads of V: row vrow, chunk 4 mb + vch, 8 bytes at 8 (gi & 1)
   const int gi = lane & 15, gg = lane >> 4;
   const int vrow = 4 * (gg >> 1) + (gi >> 2), vch = 2 * (gg & 1) + ((gi & 3) >> 1);
   uint32_t vaddr[4];
 #pragma unroll
   for (int mb = 0; mb < 4; ++mb)
-    vaddr[mb] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + BLK + vrow * D * 2 +
-                ((4 * (mb % MB) + vch) ^ (vrow & 7)) * 16 + 8 * (gi & 1);
+    vaddr[mb] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + BUF + (ks * KB + vrow) * D * 2 +
+                ((4 * (mb % MB) + vch) ^ swz<D>(vrow)) * 16 + 8 * (gi & 1);
 
-  if (bl.n > 0) issue(0);
+  if (steps > 0) issue(0);
 #pragma unroll 1
-  for (int i = 0; i < bl.n; ++i) {
+  for (int i = 0; i < steps; ++i) {
     wait_vm_lds<0>();                 // this wave's copies have landed, its reads of the other buffer are done
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const int has_i = (int)(has >> (4 * (i & 15))) & 15;
-    if (i + 1 < bl.n) {
-      if (((i + 1) & 15) == 0) {
+    const int has_i = (int)(has >> (8 * (i & 7) + ks * PPB)) & ((1 << PPB) - 1);
+    if (i + 1 < steps) {
+      if (((i + 1) & 7) == 0) {
         held = pages_from(i + 1);
         has = __builtin_amdgcn_ballot_w64(held >= 0);
       }
       issue(i + 1);
     }
-    const int key0 = block_at(i) * PKB;
+    const int t = i * NS + ks, key0 = key_of(t);
     // blocks that no row of the wave sees
-    if (key0 > whi || (g.window > 0 && key0 >= g.sinks && key0 + PKB <= wlo - g.window + 1)) continue;
-    const char* K = smem + (i & 1) * 2 * BLK;
-    float sc[32];
+    if (t >= bl.n || key0 > whi || (g.window > 0 && key0 >= g.sinks && key0 + KB <= wlo - g.window + 1)) continue;
+    const char* K = smem + (i & 1) * 2 * BUF + ks * KB * D * 2;
+    float sc[16 * NU];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < NU; ++u) {
       f32x16 a;
 #pragma unroll
       for (int e = 0; e < 16; ++e) a[e] = 0.0f;
 #pragma unroll
       for (int s = 0; s < KS; ++s)
-        a = E::mma32(*reinterpret_cast<const u32x4*>(K + (32 * u + c) * D * 2 + ((2 * s + hf) ^ (c & 7)) * 16), q[s], a);
+        a = E::mma32(*reinterpret_cast<const u32x4*>(K + (32 * u + c) * D * 2 + ((2 * s + hf) ^ swz<D>(c)) * 16), q[s], a);
 #pragma unroll
       for (int e = 0; e < 16; ++e) sc[16 * u + e] = a[e];
     }
-    const bool all = has_i == 15 && key0 + PKB - 1 <= wlo && (g.window == 0 || key0 > whi - g.window || key0 + PKB <= g.sinks);
+    const bool all = has_i == (1 << PPB) - 1 && key0 + KB - 1 <= wlo &&
+                     (g.window == 0 || key0 > whi - g.window || key0 + KB <= g.sinks);
     if (!all) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int in = 32 * u + 8 * (e >> 2) + 4 * hf + (e & 3), key = key0 + in;
-          const bool seen = (((has_i >> (in >> 4)) & 1) != 0) & (key <= pos) & ((key >= first_key) | (key < g.sinks));
-          sc[16 * u + e] = seen ? sc[16 * u + e] : -INFINITY;
-        }
+      for (int e = 0; e < 16 * NU; ++e) {
+        const int in = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + 4 * hf + (e & 3), key = key0 + in;
+        const bool seen = (((has_i >> (in >> 4)) & 1) != 0) & (key <= pos) & ((key >= first_key) | (key < g.sinks));
+        sc[e] = seen ? sc[e] : -INFINITY;
+      }
     }
     float bm = sc[0];
 #pragma unroll
-    for (int e = 1; e < 32; ++e) bm = fmaxf(bm, sc[e]);
+    for (int e = 1; e < 16 * NU; ++e) bm = fmaxf(bm, sc[e]);
     bm = fmaxf(bm, xlane_f<5>(bm));
     if (__builtin_amdgcn_ballot_w64(bm > m + 8.0f / SL) != 0ull) {
       const float mn = fmaxf(m, bm);
@@ -598,25 +612,25 @@ __global__ void __launch_bounds__(64 * PWV, 2) prefill_kernel(const AttnArgs g) 
     const float nm = m == -INFINITY ? 0.0f : -m * SL;
     float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
+    for (int e = 0; e < 16 * NU; ++e) {
       sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], SL, nm));
       sum += sc[e];
     }
     l += sum;
-    uint32_t va[4];
+    uint32_t va[4], vb[4];
 #pragma unroll
-    for (int mb = 0; mb < 4; ++mb) va[mb] = vaddr[mb] + (i & 1) * 2 * BLK;
+    for (int mb = 0; mb < 4; ++mb) {
+      va[mb] = vaddr[mb] + (i & 1) * 2 * BUF;
+      vb[mb] = va[mb] ^ (swz<D>(8) * 16);       // rows 8 further: their chunks' positions
+    }
     auto pv = [&](auto kk_) QTTS_PG_INLINE {
       constexpr int kk = decltype(kk_)::value;
       u32x4 p;
 #pragma unroll
       for (int j = 0; j < 4; ++j) p[j] = E::pack(sc[8 * kk + 2 * j], sc[8 * kk + 2 * j + 1]);
       u32x2 a[4], bq[4];
-      if constexpr (D == 128) {
-        tr_read8<16 * kk * D * 2, 8 * D * 2>(va, a, bq);
-      } else {
-        tr_read4<16 * kk * D * 2, 8 * D * 2>(va, a, bq);
-      }
+      if constexpr (D == 128) tr_read8<16 * kk * D * 2, 16 * kk * D * 2 + 8 * D * 2>(va, vb, a, bq);
+      else tr_read4<16 * kk * D * 2, 16 * kk * D * 2 + 8 * D * 2>(va, vb, a, bq);
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
         const u32x4 v = {a[mb][0], a[mb][1], bq[mb][0], bq[mb][1]};
@@ -625,40 +639,84 @@ __global__ void __launch_bounds__(64 * PWV, 2) prefill_kernel(const AttnArgs g) 
     };
     pv(std::integral_constant<int, 0>{});
     pv(std::integral_constant<int, 1>{});
-    pv(std::integral_constant<int, 2>{});
-    pv(std::integral_constant<int, 3>{});
+    if constexpr (NU == 2) {
+      pv(std::integral_constant<int, 2>{});
+      pv(std::integral_constant<int, 3>{});
+    }
   }
   l += xlane_f<5>(l);
 
-  // O^T: column = row c, register e of block mb = channel 32 mb + 8 (e >> 2) + 4 hf + (e & 3)
-  const float rl = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t* op = g.out + (long long)(at.first + ti) * g.o_token + (long long)head * g.o_head + 4 * hf;
-  float worst = 0.0f;
+  // join the splits: M = max m_s, L = sum l_s e^(m_s - M), O = sum O_s e^(m_s - M), in key order; wave (ks, wr)
+  // finishes channels ks D / NS .. of its rows
+  float* sml = reinterpret_cast<float*>(smem + 4 * BUF) + wr * NS * 2 * 32;
+  if (hf == 0) {
+    sml[(2 * ks) * 32 + c] = m;
+    sml[(2 * ks + 1) * 32 + c] = l;
+  }
+  __syncthreads();                    // every buffer is dead
+  float M = -INFINITY, L = 0.0f;
+#pragma unroll
+  for (int v = 0; v < NS; ++v) M = fmaxf(M, sml[2 * v * 32 + c]);
+#pragma unroll
+  for (int v = 0; v < NS; ++v) {
+    const float mv = sml[2 * v * 32 + c], lv = sml[(2 * v + 1) * 32 + c];
+    L += mv == -INFINITY ? lv : lv * __builtin_amdgcn_exp2f((mv - M) * SL);   // (-inf: 0, or NaN after NaN scores)
+  }
+  const float sw = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - M) * SL);
+  // [row group][split][channel block][register quad][lane][4]; O^T: column = row c, register e of block mb =
+  // channel 32 mb + 8 (e >> 2) + 4 hf + (e & 3)
+  float* so = reinterpret_cast<float*>(smem) + wr * NS * MB * 1024;
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      o[mb][e] *= rl;
-      worst += o[mb][e] - o[mb][e];   // NaN when one is not finite
+    for (int e = 0; e < 4; ++e) {
+      f32x4 x;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[k] = o[mb][4 * e + k] * sw;
+      *reinterpret_cast<f32x4*>(so + ((ks * MB + mb) * 4 + e) * 256 + lane * 4) = x;
     }
-  worst += xlane_f<5>(worst);
-  uint64_t again = __builtin_amdgcn_ballot_w64(stored && !(worst == 0.0f)) & 0xffffffffull;
-  if (stored && worst == 0.0f) {
+  __syncthreads();
+  const float rl = L == 0.0f ? 0.0f : 1.0f / L;
+  uint16_t* op = g.out + (long long)(at.first + ti) * g.o_token + (long long)head * g.o_head + 4 * hf;
+  constexpr int NQ = MB * 4 / NS;     // register quads that this wave finishes
+  f32x4 y[NQ];
+  uint32_t worst = 0u;                // largest magnitude by its bits (x - x would be contracted with the product)
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
+  for (int j = 0; j < NQ; ++j) {
+    const int e = ks * NQ + j;
+    y[j] = *reinterpret_cast<const f32x4*>(so + e * 256 + lane * 4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        u32x2 p;
-        p[0] = E::pack(o[mb][4 * e], o[mb][4 * e + 1]);
-        p[1] = E::pack(o[mb][4 * e + 2], o[mb][4 * e + 3]);
-        *reinterpret_cast<u32x2*>(op + 32 * mb + 8 * e) = p;
-      }
+    for (int v = 1; v < NS; ++v) y[j] += *reinterpret_cast<const f32x4*>(so + (v * MB * 4 + e) * 256 + lane * 4);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      y[j][k] *= rl;
+      worst = max(worst, __float_as_uint(y[j][k]) & 0x7fffffffu);
+    }
   }
-  while (again != 0ull) {
+  worst = max(worst, xlane<5>(worst));
+  // rows that are to be summed again, known to every split (their words are free again: all have read them)
+  __syncthreads();
+  if (hf == 0) sml[2 * ks * 32 + c] = __uint_as_float(worst);
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < NS; ++v) worst = max(worst, __float_as_uint(sml[2 * v * 32 + c]));
+  if (stored && worst < 0x7f800000u) {
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+      const int e = ks * NQ + j;
+      u32x2 p;
+      p[0] = E::pack(y[j][0], y[j][1]);
+      p[1] = E::pack(y[j][2], y[j][3]);
+      *reinterpret_cast<u32x2*>(op + 8 * e) = p;
+    }
+  }
+  uint64_t again = __builtin_amdgcn_ballot_w64(stored && worst >= 0x7f800000u) & 0xffffffffull;
+  for (int n = 0; again != 0ull; ++n) {        // the splits take them in turn
     const int src = __builtin_ctzll(again);
     again &= again - 1;
-    exact_row<E, D>(g, at.b, kvh, at.first + __builtin_amdgcn_readlane(ti, src), __builtin_amdgcn_readlane(head, src),
-                    __builtin_amdgcn_readlane(pos, src));
+    if (n % NS == ks)
+      exact_row<E, D>(g, at.b, kvh, at.first + __builtin_amdgcn_readlane(ti, src), __builtin_amdgcn_readlane(head, src),
+                      __builtin_amdgcn_readlane(pos, src));
   }
 }
 
@@ -720,6 +778,22 @@ void launch_decode(const AttnArgs& g, hipStream_t st) {
   hipLaunchKernelGGL((decode_kernel<E, D>), dim3((unsigned)((long long)g.requests * g.hkv * tiles * g.splits)), dim3(64 * DW), 0, st, g);
   if (g.splits > 1)
     hipLaunchKernelGGL((decode_join_kernel<E, D>), dim3((unsigned)(((long long)g.requests * g.hq + 3) / 4)), dim3(256), 0, st, g);
+}
+
+template <class E, int D, int NS>
+hipError_t launch_prefill(const AttnArgs& g, hipStream_t st) {
+  constexpr int PM = 32 * PWV / NS;
+  // every request ends with a tile that may be part empty; no more tiles than rows
+  const long long n = (long long)g.tokens * g.group, tiles = std::min(n / PM + g.requests, n);
+  if (tiles * g.hkv > INT_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((prefill_kernel<E, D, NS>), dim3((unsigned)(tiles * g.hkv)), dim3(64 * PWV), 0, st, g);
+  return hipGetLastError();
+}
+template <class E, int D>
+hipError_t prefill_split(const AttnArgs& g, hipStream_t st) {
+  static const char* e = getenv("QNS");
+  if (e && e[0] == '4') return launch_prefill<E, D, 4>(g, st);
+  return launch_prefill<E, D, 2>(g, st);
 }
 
 }  // namespace pg
@@ -786,18 +860,8 @@ hipError_t qtts_paged_attention_prefill(const QttsPagedCache* cache, int n_reque
                          block_table, table_width, table_stride, kv_lens, n_requests, scale, window, sinks);
   g.cu = cu_tokens;
   g.tokens = n_tokens;
-  // every request ends with a tile that may be part empty; no more tiles than rows
-  const long long tiles = std::min((long long)n_tokens * g.group / PM + n_requests, (long long)n_tokens * g.group);
-  if (tiles * g.hkv > INT_MAX) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)(tiles * g.hkv)), block(64 * PWV);
-  if (cache->dtype == QTTS_BF16) {
-    if (cache->head_dim == 128) hipLaunchKernelGGL((prefill_kernel<Bf16, 128>), grid, block, 0, stream, g);
-    else hipLaunchKernelGGL((prefill_kernel<Bf16, 64>), grid, block, 0, stream, g);
-  } else {
-    if (cache->head_dim == 128) hipLaunchKernelGGL((prefill_kernel<F16, 128>), grid, block, 0, stream, g);
-    else hipLaunchKernelGGL((prefill_kernel<F16, 64>), grid, block, 0, stream, g);
-  }
-  return hipGetLastError();
+  if (cache->dtype == QTTS_BF16) return cache->head_dim == 128 ? prefill_split<Bf16, 128>(g, stream) : prefill_split<Bf16, 64>(g, stream);
+  return cache->head_dim == 128 ? prefill_split<F16, 128>(g, stream) : prefill_split<F16, 64>(g, stream);
 }
 
 }  // extern "C"
