@@ -351,8 +351,8 @@ hipError_t qtts_cp_frame_shared(
 enum { QTTS_BF16 = 0, QTTS_F16 = 1 };
 
 /* One layer's pages. Element (page, head, place, channel) of K (and of V) is at page * page_stride +
- * head * head_stride + place * slot_stride + channel; strides in elements, multiples of 8 (page and
- * head strides up to 2^31 - 1 for a head, slot strides up to 2^24), k and v 16-byte aligned.
+ * head * head_stride + place * slot_stride + channel; strides in elements, multiples of 8
+ * (page and head strides below 2^31, slot strides up to 2^24), k and v 16-byte aligned.
  * page_size: a power of two, 16 .. 65536. head_dim: 64 or 128. */
 typedef struct QttsPagedCache {
     void* k;

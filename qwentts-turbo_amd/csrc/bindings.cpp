@@ -680,7 +680,7 @@ QttsPagedCache paged_cache(const Tensor& k, const Tensor& v) {
   TORCH_CHECK(k.size(0) >= 1 && k.size(0) <= INT_MAX && k.size(1) >= 1 && k.size(1) <= INT_MAX, "empty cache: ", k.sizes());
   TORCH_CHECK(k.stride(3) == 1, "the cache's channels must be contiguous");
   for (int i = 0; i < 3; ++i) TORCH_CHECK(k.stride(i) >= 0 && k.stride(i) % 8 == 0, "cache strides must be multiples of 8, got ", k.strides());
-  TORCH_CHECK(k.stride(2) >= k.size(3) && k.stride(2) <= (1 << 24) && k.stride(1) <= INT_MAX, "cache strides out of range: ", k.strides());
+  TORCH_CHECK(k.stride(2) >= k.size(3) && k.stride(2) <= (1 << 24) && k.stride(1) <= INT_MAX && k.stride(0) <= INT_MAX, "cache strides out of range: ", k.strides());
   check_aligned(k, "k_cache");
   check_aligned(v, "v_cache");
   QttsPagedCache c;

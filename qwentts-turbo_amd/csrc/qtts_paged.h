@@ -47,8 +47,7 @@ struct F16 {
 struct Pages {
   const uint16_t* k;
   const uint16_t* v;
-  long long page_stride;
-  int head_stride, slot_stride;
+  int page_stride, head_stride, slot_stride;
   int num_pages, shift;      // page size = 1 << shift
 };
 
@@ -62,11 +61,11 @@ inline bool cache_ok(const QttsPagedCache* c) {
   if (c->page_size < 16 || c->page_size > 65536 || (c->page_size & (c->page_size - 1)) != 0) return false;
   if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15u) != 0) return false;
   if (((c->page_stride | c->head_stride | c->slot_stride) & 7) != 0) return false;
-  if (c->page_stride < 0 || c->head_stride < 0 || c->head_stride > 0x7fffffffLL) return false;
+  if (c->page_stride < 0 || c->page_stride > 0x7fffffffLL || c->head_stride < 0 || c->head_stride > 0x7fffffffLL) return false;
   return c->slot_stride >= c->head_dim && c->slot_stride <= (1 << 24);
 }
 inline Pages pages_of(const QttsPagedCache* c) {
-  return Pages{static_cast<const uint16_t*>(c->k), static_cast<const uint16_t*>(c->v), c->page_stride,
+  return Pages{static_cast<const uint16_t*>(c->k), static_cast<const uint16_t*>(c->v), (int)c->page_stride,
                (int)c->head_stride, (int)c->slot_stride, c->num_pages, __builtin_ctz((unsigned)c->page_size)};
 }
 

@@ -72,26 +72,35 @@ __device__ __forceinline__ int swz(int r) {
   else return ((r << 1) & 4) | ((r >> 1) & 2) | ((r >> 3) & 1);
 }
 
-// One 16-key piece of K and V into LDS by DMA. The descriptors begin at the piece's first row and end with its last, and rows that are
-// not `seen` are asked for past the end: they come as zeros.
-template <int D, class Seen>
-__device__ __forceinline__ void copy_piece(const Pages& pg, int page, int key0, int kvh, char* k_dst, char* v_dst, int lane,
-                                           Seen&& seen) {
-  constexpr int CPR = D / 8, RPI = 64 / CPR;           // chunks a row, rows an instruction
-  const long long at = (long long)page * pg.page_stride + (long long)kvh * pg.head_stride +
-                       (long long)(key0 & ((1 << pg.shift) - 1)) * pg.slot_stride;
-  const int bytes = (15 * pg.slot_stride + D) * 2;
-  const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(pg.k + at), (short)0, bytes, 0x00020000);
-  const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(pg.v + at), (short)0, bytes, 0x00020000);
+// 16-key pieces of K or V into LDS by DMA. The descriptor begins at the piece's first row and ends with its last.
+// A piece whose rows are not all seen asks for the others past the end: they come as zeros. The lane's offsets
+// inside a piece are the same for all of them.
+template <int D>
+struct PieceCopy {
+  static constexpr int CPR = D / 8, RPI = 64 / CPR, N = 16 / RPI;   // chunks a row, rows an instruction, instructions
+  int off[N];
+  __device__ __forceinline__ PieceCopy(int slot_stride, int lane) {
 #pragma unroll
-  for (int i = 0; i < 16 / RPI; ++i) {
-    const int r = RPI * i + lane / CPR;
-    const int in = r * pg.slot_stride * 2 + ((lane % CPR) ^ swz<D>(r)) * 16;
-    const int off = seen(key0 + r) ? in : 0x7fffff00;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lvoid_t*)(k_dst + i * 1024), 16, off, 0, 0, 0);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lvoid_t*)(v_dst + i * 1024), 16, off, 0, 0, 0);
+    for (int i = 0; i < N; ++i) {
+      const int r = RPI * i + lane / CPR;
+      off[i] = r * slot_stride * 2 + ((lane % CPR) ^ swz<D>(r)) * 16;
+    }
   }
-}
+  // the piece's descriptor; `head`: the KV head's channels in page 0
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t piece(const uint16_t* head, const Pages& pg, int page, int key0) const {
+    const long long at = (long long)page * pg.page_stride + (long long)((key0 & ((1 << pg.shift) - 1)) * (long long)pg.slot_stride);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(head + at), (short)0, (15 * pg.slot_stride + D) * 2, 0x00020000);
+  }
+  // the lane's offsets in a piece of which only the rows that seen(key) says are wanted
+  template <class Seen>
+  __device__ __forceinline__ void some(int key0, int lane, int (&o)[N], Seen&& seen) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = seen(key0 + RPI * i + lane / CPR) ? off[i] : 0x7fffff00;
+  }
+  __device__ __forceinline__ static void one(__amdgpu_buffer_rsrc_t rs, char* dst, int o) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lvoid_t*)dst, 16, o, 0, 0, 0);
+  }
+};
 
 // ---- decode --------------------------------------------------------------------------------
 // One workgroup of 4 waves per (request, KV head, up to 16 of its query heads, part of its keys). Bound by
@@ -125,17 +134,24 @@ __device__ __forceinline__ void tr_read8(const uint32_t (&a)[4], const uint32_t 
       : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]), "i"(A), "i"(B)
       : "memory");
 }
-template <int A, int B>
-__device__ __forceinline__ void tr_read4(const uint32_t (&a)[4], const uint32_t (&b)[4], u32x2 (&lo)[4], u32x2 (&hi)[4]) {
+// two MFMA steps (the second S bytes further)
+template <int A, int B, int S>
+__device__ __forceinline__ void tr_read16(const uint32_t (&a)[4], const uint32_t (&b)[4], u32x2 (&lo)[8], u32x2 (&hi)[8]) {
   asm volatile(
-      "ds_read_b64_tr_b16 %0, %4 offset:%c8\n\tds_read_b64_tr_b16 %2, %6 offset:%c9\n\t"
-      "ds_read_b64_tr_b16 %1, %5 offset:%c8\n\tds_read_b64_tr_b16 %3, %7 offset:%c9\n\t"
+      "ds_read_b64_tr_b16 %0, %16 offset:%c24\n\tds_read_b64_tr_b16 %8, %20 offset:%c25\n\t"
+      "ds_read_b64_tr_b16 %1, %17 offset:%c24\n\tds_read_b64_tr_b16 %9, %21 offset:%c25\n\t"
+      "ds_read_b64_tr_b16 %2, %18 offset:%c24\n\tds_read_b64_tr_b16 %10, %22 offset:%c25\n\t"
+      "ds_read_b64_tr_b16 %3, %19 offset:%c24\n\tds_read_b64_tr_b16 %11, %23 offset:%c25\n\t"
+      "ds_read_b64_tr_b16 %4, %16 offset:%c26\n\tds_read_b64_tr_b16 %12, %20 offset:%c27\n\t"
+      "ds_read_b64_tr_b16 %5, %17 offset:%c26\n\tds_read_b64_tr_b16 %13, %21 offset:%c27\n\t"
+      "ds_read_b64_tr_b16 %6, %18 offset:%c26\n\tds_read_b64_tr_b16 %14, %22 offset:%c27\n\t"
+      "ds_read_b64_tr_b16 %7, %19 offset:%c26\n\tds_read_b64_tr_b16 %15, %23 offset:%c27\n\t"
       "s_waitcnt lgkmcnt(0)"
-      : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(hi[0]), "=&v"(hi[1])
-      : "v"(a[0]), "v"(a[1]), "v"(b[0]), "v"(b[1]), "i"(A), "i"(B)
+      : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(lo[2]), "=&v"(lo[3]), "=&v"(lo[4]), "=&v"(lo[5]), "=&v"(lo[6]), "=&v"(lo[7]),
+        "=&v"(hi[0]), "=&v"(hi[1]), "=&v"(hi[2]), "=&v"(hi[3]), "=&v"(hi[4]), "=&v"(hi[5]), "=&v"(hi[6]), "=&v"(hi[7])
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]), "i"(A), "i"(B), "i"(A + S), "i"(B + S)
       : "memory");
 }
-
 template <class E, int D>
 __global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
   constexpr int BLK = DKB * D * 2;               // bytes of a K or V block
@@ -178,14 +194,28 @@ __global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
   };
   int held = pages_from(0), next_held = 0;
   uint64_t has = __builtin_amdgcn_ballot_w64(held >= 0);      // of block i: bits 2 (i & 31), + 1
+  const PieceCopy<D> copy(g.pages.slot_stride, lane);
+  const uint16_t* const k_head = g.pages.k + (long long)kvh * g.pages.head_stride;
+  const uint16_t* const v_head = g.pages.v + (long long)kvh * g.pages.head_stride;
   auto issue = [&](int i) QTTS_PG_INLINE {
     const int kb = block_at(i);
     char* dst = buf + (i & 1) * 2 * BLK;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int page = __builtin_amdgcn_readlane(held, 2 * (i & 31) + u);
-      copy_piece<D>(g.pages, max(page, 0), kb * DKB + 16 * u, kvh, dst + u * 16 * D * 2, dst + BLK + u * 16 * D * 2, lane,
-                    [&](int key) QTTS_PG_INLINE { return (page >= 0) & (key < len) & ((key >= lo) | (key < g.sinks)); });
+      const int k0 = kb * DKB + 16 * u;
+      const bool whole = page >= 0 && k0 + 16 <= len && (k0 >= lo || k0 + 16 <= g.sinks);
+      auto seen = [&](int key) QTTS_PG_INLINE { return (page >= 0) & (key < len) & ((key >= lo) | (key < g.sinks)); };
+      const auto kr = copy.piece(k_head, g.pages, max(page, 0), k0), vr = copy.piece(v_head, g.pages, max(page, 0), k0);
+      int off[copy.N];
+#pragma unroll
+      for (int j = 0; j < copy.N; ++j) off[j] = copy.off[j];
+      if (!whole) copy.some(k0, lane, off, seen);
+#pragma unroll
+      for (int j = 0; j < copy.N; ++j) {
+        copy.one(kr, dst + u * 16 * D * 2 + j * 1024, off[j]);
+        copy.one(vr, dst + BLK + u * 16 * D * 2 + j * 1024, off[j]);
+      }
     }
   };
 
@@ -523,20 +553,63 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
 
   const int* row = g.table + (long long)at.b * g.table_stride;
   auto key_of = [&](int t) QTTS_PG_INLINE { return (t < bl.ns ? t : t + bl.skip) * KB; };   // first key of block t
-  // pages of 8 steps, one 16-key piece a lane (-1: none)
-  auto pages_from = [&](int i0) QTTS_PG_INLINE {
-    const int t = (i0 + (lane >> 3)) * NS + (lane & 7) / PPB, key = key_of(t) + 16 * (lane & (PPB - 1));
-    int p = -1;
-    if (t < bl.n && key < end) p = *gmem(row + (key >> g.pages.shift));
-    return (unsigned)p < (unsigned)g.pages.num_pages ? p : -1;
+  // The table entries of a step's 8 pieces, piece lane & 7 a lane, loaded a step before they are used; in: the pieces
+  // that have keys, as bits.
+  struct Entries {
+    int e;
+    uint32_t in;
   };
-  int held = pages_from(0);
-  uint64_t has = __builtin_amdgcn_ballot_w64(held >= 0);
-  auto issue = [&](int i) QTTS_PG_INLINE {                   // wave w copies piece w of the step
-    const int page = __builtin_amdgcn_readlane(held, 8 * (i & 7) + w);
-    char* dst = smem + (i & 1) * 2 * BUF + w * 16 * D * 2;
-    copy_piece<D>(g.pages, max(page, 0), key_of(i * NS + w / PPB) + 16 * (w % PPB), kvh, dst, dst + BUF, lane,
-                  [&](int key) QTTS_PG_INLINE { return (page >= 0) & (key < end) & ((key >= lo) | (key < g.sinks)); });
+  auto entries = [&](int i) QTTS_PG_INLINE {
+    const int t = i * NS + (lane & 7) / PPB, key = key_of(t) + 16 * (lane & (PPB - 1));
+    const bool in = (t < bl.n) & (key < end);
+    return Entries{*gmem(row + (in ? key >> g.pages.shift : 0)), (uint32_t)__builtin_amdgcn_ballot_w64(in) & 255u};
+  };
+  // pieces with a page of the cache, as bits; and the page of this wave's (-1: none)
+  auto found = [&](const Entries& x) QTTS_PG_INLINE {
+    return (uint32_t)__builtin_amdgcn_ballot_w64((unsigned)x.e < (unsigned)g.pages.num_pages) & x.in;
+  };
+  auto own = [&](const Entries& x, uint32_t has) QTTS_PG_INLINE {
+    const int page = __builtin_amdgcn_readlane(x.e, w), none = (int)((has >> w) & 1) - 1;   // -1: none
+    return page | none;
+  };
+  // steps whose wave's block is seen whole by all its rows, and whose copies (this wave's pieces of V a step and of K
+  // two steps on) are whole: no mask, no partial piece
+  int fs, fe;
+  {
+    const int see0 = g.window > 0 ? max(bl.ns, (max(whi - g.window + 1, 0) + KB - 1) / KB - bl.skip) : 0;
+    const int see1 = (max(wlo, -1) + 1) / KB - bl.skip, copy1 = end / KB - bl.skip;
+    const int copy0 = g.window > 0 ? max(bl.ns, (lo + KB - 1) / KB - bl.skip) : 0;
+    fs = (max(max(see0, copy0) - ks, 0) + NS - 1) / NS;
+    fe = (max(min(see1, copy1 - NS) - ks, 0) + NS - 1) / NS;
+  }
+  const PieceCopy<D> copy(g.pages.slot_stride, lane);
+  const uint16_t* const k_head = g.pages.k + (long long)kvh * g.pages.head_stride;
+  const uint16_t* const v_head = g.pages.v + (long long)kvh * g.pages.head_stride;
+  // The copy of piece w of step i by wave w: K's into half 0 of its buffer, V's into half 1.
+  struct Piece {
+    __amdgpu_buffer_rsrc_t rs;
+    char* dst;
+    int key0, page;
+    int off[PieceCopy<D>::N];
+  };
+  auto piece = [&](const uint16_t* head, int page, int i, int half) QTTS_PG_INLINE {
+    Piece p;
+    p.page = page;
+    p.key0 = key_of(i * NS + w / PPB) + 16 * (w % PPB);
+    p.rs = copy.piece(head, g.pages, max(page, 0), p.key0);
+    p.dst = smem + (i & 1) * 2 * BUF + half * BUF + w * 16 * D * 2;
+#pragma unroll
+    for (int j = 0; j < copy.N; ++j) p.off[j] = copy.off[j];
+    return p;
+  };
+  auto part = [&](Piece& p) QTTS_PG_INLINE {             // only the rows that are seen
+    copy.some(p.key0, lane, p.off,
+              [&](int key) QTTS_PG_INLINE { return (p.page >= 0) & (key < end) & ((key >= lo) | (key < g.sinks)); });
+  };
+  auto issue = [&](Piece p) QTTS_PG_INLINE {
+    part(p);
+#pragma unroll
+    for (int j = 0; j < copy.N; ++j) copy.one(p.rs, p.dst + j * 1024, p.off[j]);
   };
 
   const float SL = g.scale_log2;
@@ -555,46 +628,80 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
     vaddr[mb] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + BUF + (ks * KB + vrow) * D * 2 +
                 ((4 * (mb % MB) + vch) ^ swz<D>(vrow)) * 16 + 8 * (gi & 1);
 
-  if (steps > 0) issue(0);
-#pragma unroll 1
-  for (int i = 0; i < steps; ++i) {
-    wait_vm_lds<0>();                 // this wave's copies have landed, its reads of the other buffer are done
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    const int has_i = (int)(has >> (8 * (i & 7) + ks * PPB)) & ((1 << PPB) - 1);
-    if (i + 1 < steps) {
-      if (((i + 1) & 7) == 0) {
-        held = pages_from(i + 1);
-        has = __builtin_amdgcn_ballot_w64(held >= 0);
-      }
-      issue(i + 1);
+  float sc[16 * NU];
+  u32x4 p[2 * NU];
+  // K fragments of half of the channel steps, of the block's NU score blocks: h = 0, 1
+  u32x4 kf[2][NU][KS / 2];
+  auto read_k = [&](int i, int h) QTTS_PG_INLINE {
+    const char* K = smem + (i & 1) * 2 * BUF + (ks * KB + c) * D * 2;
+#pragma unroll
+    for (int s = 0; s < KS / 2; ++s)
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+        kf[h][u][s] = *reinterpret_cast<const u32x4*>(K + 32 * u * D * 2 + ((KS * h + 2 * s + hf) ^ swz<D>(c)) * 16);
+  };
+  // scores of step i, the first half of K's fragments read before; the blocks' sums run as chains of their own
+  auto scores = [&](int i) QTTS_PG_INLINE {
+    f32x16 a[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) a[u][e] = 0.0f;
+    read_k(i, 1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int s = 0; s < KS / 2; ++s)
+#pragma unroll
+        for (int u = 0; u < NU; ++u) a[u] = E::mma32(kf[h][u][s], q[h * KS / 2 + s], a[u]);
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[16 * u + e] = a[u][e];
+  };
+  // O^T += V^T P^T of MFMA steps kk and kk + 1 of step i
+  auto products = [&](int i, auto kk_) QTTS_PG_INLINE {
+    constexpr int kk = decltype(kk_)::value;
+    uint32_t va[4], vb[4];
+#pragma unroll
+    for (int mb = 0; mb < 4; ++mb) {
+      va[mb] = vaddr[mb] + (i & 1) * 2 * BUF;
+      vb[mb] = va[mb] ^ (swz<D>(8) * 16);       // rows 8 further: their chunks' positions
     }
-    const int t = i * NS + ks, key0 = key_of(t);
-    // blocks that no row of the wave sees
-    if (t >= bl.n || key0 > whi || (g.window > 0 && key0 >= g.sinks && key0 + KB <= wlo - g.window + 1)) continue;
-    const char* K = smem + (i & 1) * 2 * BUF + ks * KB * D * 2;
-    float sc[16 * NU];
+    if constexpr (D == 128) {
+      u32x2 a[8], bq[8];
+      tr_read16<16 * kk * D * 2, 16 * kk * D * 2 + 8 * D * 2, 16 * D * 2>(va, vb, a, bq);
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      f32x16 a;
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) a[e] = 0.0f;
+        for (int mb = 0; mb < MB; ++mb) {
+          const u32x4 v = {a[4 * j + mb][0], a[4 * j + mb][1], bq[4 * j + mb][0], bq[4 * j + mb][1]};
+          o[mb] = E::mma32(v, p[kk + j], o[mb]);
+        }
+    } else {
+      u32x2 a[4], bq[4];
+      const uint32_t xa[4] = {va[0], va[1], va[0] + 16 * D * 2, va[1] + 16 * D * 2};
+      const uint32_t xb[4] = {vb[0], vb[1], vb[0] + 16 * D * 2, vb[1] + 16 * D * 2};
+      tr_read8<16 * kk * D * 2, 16 * kk * D * 2 + 8 * D * 2>(xa, xb, a, bq);
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-        a = E::mma32(*reinterpret_cast<const u32x4*>(K + (32 * u + c) * D * 2 + ((2 * s + hf) ^ swz<D>(c)) * 16), q[s], a);
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[16 * u + e] = a[e];
+        for (int mb = 0; mb < MB; ++mb) {
+          const u32x4 v = {a[2 * j + mb][0], a[2 * j + mb][1], bq[2 * j + mb][0], bq[2 * j + mb][1]};
+          o[mb] = E::mma32(v, p[kk + j], o[mb]);
+        }
     }
-    const bool all = has_i == (1 << PPB) - 1 && key0 + KB - 1 <= wlo &&
-                     (g.window == 0 || key0 > whi - g.window || key0 + KB <= g.sinks);
-    if (!all) {
+  };
+  auto mask = [&](int i, int has_i) QTTS_PG_INLINE {
+    const int key0 = key_of(i * NS + ks);
 #pragma unroll
-      for (int e = 0; e < 16 * NU; ++e) {
-        const int in = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + 4 * hf + (e & 3), key = key0 + in;
-        const bool seen = (((has_i >> (in >> 4)) & 1) != 0) & (key <= pos) & ((key >= first_key) | (key < g.sinks));
-        sc[e] = seen ? sc[e] : -INFINITY;
-      }
+    for (int e = 0; e < 16 * NU; ++e) {
+      const int in = 32 * (e >> 4) + 8 * ((e >> 2) & 3) + 4 * hf + (e & 3), key = key0 + in;
+      const bool seen = (((has_i >> (in >> 4)) & 1) != 0) & (key <= pos) & ((key >= first_key) | (key < g.sinks));
+      sc[e] = seen ? sc[e] : -INFINITY;
     }
+  };
+  auto softmax = [&](const Piece& kp, const Piece& vp) QTTS_PG_INLINE {
     float bm = sc[0];
 #pragma unroll
     for (int e = 1; e < 16 * NU; ++e) bm = fmaxf(bm, sc[e]);
@@ -612,38 +719,55 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
     const float nm = m == -INFINITY ? 0.0f : -m * SL;
     float sum = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 16 * NU; ++e) {
-      sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], SL, nm));
-      sum += sc[e];
+    for (int j = 0; j < 8 * NU; ++j) {
+      const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[2 * j], SL, nm)), e1 = __builtin_amdgcn_exp2f(fmaf(sc[2 * j + 1], SL, nm));
+      sum += e0;
+      sum += e1;
+      p[j >> 2][j & 3] = E::pack(e0, e1);
+      // one copy at a time between the exponentials: issued together they hold the wave for 130 cycles each
+      constexpr int every = 8 * NU / (2 * copy.N);
+      if (j % every == every - 1) {
+        const int n = j / every;
+        if (n < copy.N) copy.one(kp.rs, kp.dst + n * 1024, kp.off[n]);
+        else copy.one(vp.rs, vp.dst + (n - copy.N) * 1024, vp.off[n - copy.N]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     l += sum;
-    uint32_t va[4], vb[4];
-#pragma unroll
-    for (int mb = 0; mb < 4; ++mb) {
-      va[mb] = vaddr[mb] + (i & 1) * 2 * BUF;
-      vb[mb] = va[mb] ^ (swz<D>(8) * 16);       // rows 8 further: their chunks' positions
+  };
+  auto barrier = [&]() QTTS_PG_INLINE {
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // what step i copies (step i + 1's pieces) and whether it needs masks or partial pieces
+  const Entries first = entries(0);
+  Entries second = entries(1);
+  uint32_t has = found(first);                            // of the step computed
+  issue(piece(k_head, own(first, has), 0, 0));
+  issue(piece(v_head, own(first, has), 0, 1));
+#pragma unroll 1
+  for (int i = 0; i < steps; ++i) {
+    wait_vm_lds<0>();                 // this wave's copies have landed, its reads of the other buffer are done
+    barrier();
+    read_k(i, 0);
+    const uint32_t has_n = found(second);                 // of step i + 1
+    const int page = own(second, has_n);
+    Piece kp = piece(k_head, page, i + 1, 0), vp = piece(v_head, page, i + 1, 1);
+    second = entries(i + 2);
+    const int has_i = (int)(has >> (ks * PPB)) & ((1 << PPB) - 1);
+    has = has_n;
+    const bool whole = (i >= fs) & (i < fe) & (has_i == (1 << PPB) - 1) & (page >= 0);
+    scores(i);
+    if (!whole) {
+      part(kp);
+      part(vp);
+      mask(i, has_i);
     }
-    auto pv = [&](auto kk_) QTTS_PG_INLINE {
-      constexpr int kk = decltype(kk_)::value;
-      u32x4 p;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) p[j] = E::pack(sc[8 * kk + 2 * j], sc[8 * kk + 2 * j + 1]);
-      u32x2 a[4], bq[4];
-      if constexpr (D == 128) tr_read8<16 * kk * D * 2, 16 * kk * D * 2 + 8 * D * 2>(va, vb, a, bq);
-      else tr_read4<16 * kk * D * 2, 16 * kk * D * 2 + 8 * D * 2>(va, vb, a, bq);
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        const u32x4 v = {a[mb][0], a[mb][1], bq[mb][0], bq[mb][1]};
-        o[mb] = E::mma32(v, p, o[mb]);
-      }
-    };
-    pv(std::integral_constant<int, 0>{});
-    pv(std::integral_constant<int, 1>{});
-    if constexpr (NU == 2) {
-      pv(std::integral_constant<int, 2>{});
-      pv(std::integral_constant<int, 3>{});
-    }
+    softmax(kp, vp);
+    products(i, std::integral_constant<int, 0>{});
+    if constexpr (NU == 2) products(i, std::integral_constant<int, 2>{});
   }
+  wait_vm_lds<0>();
   l += xlane_f<5>(l);
 
   // join the splits: M = max m_s, L = sum l_s e^(m_s - M), O = sum O_s e^(m_s - M), in key order; wave (ks, wr)
