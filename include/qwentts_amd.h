@@ -433,7 +433,7 @@ hipError_t qtts_paged_attention_prefill(
     const QttsPagedCache* cache, int n_requests, int n_tokens, int num_q_heads, const void* q,
     long long q_token_stride, long long q_head_stride, void* out, long long out_token_stride,
     long long out_head_stride, const int* block_table, int table_width, long long table_stride,
-    const int* kv_lens, const int* cu_tokens, float scale, int window, int sinks, hipStream_t stream);
+    const int* kv_lens, const int* cu_tokens, int max_len, float scale, int window, int sinks, hipStream_t stream);
 
 /* Debugging aid (no reference counterpart): record the weight-shared kernels' step timeline
  * (s_memrealtime stamps, [256 workgroups][1024 steps][16]: after the entry barrier, after the

@@ -872,7 +872,7 @@ Tensor paged_attention_prefill(Tensor q, Tensor k_cache, Tensor v_cache, Tensor 
   hip_check(qtts_paged_attention_prefill(&cache, (int)n, (int)q.size(0), (int)q.size(1), q.data_ptr(), tok_stride(q), head_stride(q),
                                          o.data_ptr(), tok_stride(o), head_stride(o), block_table.data_ptr<int>(),
                                          (int)block_table.size(1), table_stride(block_table), kv_lens.data_ptr<int>(), cu,
-                                         (float)scale, (int)window, (int)sinks, cur_stream()),
+                                         (int)std::min<int64_t>(max_len, INT_MAX), (float)scale, (int)window, (int)sinks, cur_stream()),
             "qtts_paged_attention_prefill");
   return o;
 }

@@ -427,7 +427,6 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const AttnArgs g) {
 // row of a tile and seen by another: rows that end with a number that is not finite are summed again over
 // the keys that they see, one by one (exact_row).
 constexpr int PWV = 8;                // waves
-constexpr int PSTEP = 128;            // keys of a step
 
 // Row `r` of (request b, KV head kvh) again, key by key: the wave's lanes take D / 64 channels each.
 template <class E, int D>
@@ -521,11 +520,15 @@ __device__ __forceinline__ TilePlace find_tile(const AttnArgs& g, int back) {
 
 template <class E, int D, int NS>
 __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(const AttnArgs g) {
-  constexpr int NR = PWV / NS, PM = 32 * NR, KB = PSTEP / NS;   // rows of a tile, keys of a wave's block
-  constexpr int NU = KB / 32, PPB = KB / 16;                    // 32-key score blocks, pieces of a block
-  constexpr int BUF = PSTEP * D * 2;                            // bytes of a step's K or V
+  constexpr int NR = PWV / NS, PM = 32 * NR, KB = NS == 4 ? 32 : 64;   // row groups, rows of a tile, keys of a wave's block
+  constexpr int STEP = NS * KB, NP = STEP / 16;                        // keys of a step, its pieces (8, or 4)
+  constexpr int NU = KB / 32, PPB = KB / 16;                           // 32-key score blocks, pieces of a block
+  constexpr int BUF = STEP * D * 2;                                    // bytes of a step's K or V
+  constexpr int PAIR = NP / 4;                                         // pieces that a wave copies: K and V, or one of them
   constexpr int MB = D / 32, KS = D / 16;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * BUF + PWV * 2 * 32 * 4];   // (K, V) x 2 buffers; (m, l) of the join
+  constexpr int JOIN = PWV * D * 32 * 4;                               // bytes of the join's sums (one split needs none)
+  constexpr int ROOM = NS > 1 && JOIN > 4 * BUF ? JOIN : 4 * BUF;
+  __shared__ __attribute__((aligned(1024))) char smem[ROOM + PWV * 2 * 32 * 4];   // (K, V) x 2 buffers; (m, l) of the join
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int hf = lane >> 5, c = lane & 31, wr = w % NR, ks = w / NR;
   const int kvh = blockIdx.x % g.hkv;
@@ -553,23 +556,23 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
 
   const int* row = g.table + (long long)at.b * g.table_stride;
   auto key_of = [&](int t) QTTS_PG_INLINE { return (t < bl.ns ? t : t + bl.skip) * KB; };   // first key of block t
-  // The table entries of a step's 8 pieces, piece lane & 7 a lane, loaded a step before they are used; in: the pieces
+  // The table entries of a step's pieces, piece lane & (NP - 1) a lane, loaded a step before they are used; in: the pieces
   // that have keys, as bits.
   struct Entries {
     int e;
     uint32_t in;
   };
   auto entries = [&](int i) QTTS_PG_INLINE {
-    const int t = i * NS + (lane & 7) / PPB, key = key_of(t) + 16 * (lane & (PPB - 1));
+    const int t = i * NS + (lane & (NP - 1)) / PPB, key = key_of(t) + 16 * (lane & (PPB - 1));
     const bool in = (t < bl.n) & (key < end);
-    return Entries{*gmem(row + (in ? key >> g.pages.shift : 0)), (uint32_t)__builtin_amdgcn_ballot_w64(in) & 255u};
+    return Entries{*gmem(row + (in ? key >> g.pages.shift : 0)), (uint32_t)__builtin_amdgcn_ballot_w64(in) & ((1u << NP) - 1)};
   };
   // pieces with a page of the cache, as bits; and the page of this wave's (-1: none)
   auto found = [&](const Entries& x) QTTS_PG_INLINE {
     return (uint32_t)__builtin_amdgcn_ballot_w64((unsigned)x.e < (unsigned)g.pages.num_pages) & x.in;
   };
   auto own = [&](const Entries& x, uint32_t has) QTTS_PG_INLINE {
-    const int page = __builtin_amdgcn_readlane(x.e, w), none = (int)((has >> w) & 1) - 1;   // -1: none
+    const int page = __builtin_amdgcn_readlane(x.e, w % NP), none = (int)((has >> (w % NP)) & 1) - 1;   // -1: none
     return page | none;
   };
   // steps whose wave's block is seen whole by all its rows, and whose copies (this wave's pieces of V a step and of K
@@ -585,7 +588,8 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
   const PieceCopy<D> copy(g.pages.slot_stride, lane);
   const uint16_t* const k_head = g.pages.k + (long long)kvh * g.pages.head_stride;
   const uint16_t* const v_head = g.pages.v + (long long)kvh * g.pages.head_stride;
-  // The copy of piece w of step i by wave w: K's into half 0 of its buffer, V's into half 1.
+  // The copy of a piece of step i by wave w, of K into half 0 of its buffer or of V into half 1: piece w of both, or, of
+  // a step of 4 pieces, piece w % 4 of K (waves 0 .. 3) or V.
   struct Piece {
     __amdgpu_buffer_rsrc_t rs;
     char* dst;
@@ -595,9 +599,9 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
   auto piece = [&](const uint16_t* head, int page, int i, int half) QTTS_PG_INLINE {
     Piece p;
     p.page = page;
-    p.key0 = key_of(i * NS + w / PPB) + 16 * (w % PPB);
+    p.key0 = key_of(i * NS + w % NP / PPB) + 16 * (w % PPB);
     p.rs = copy.piece(head, g.pages, max(page, 0), p.key0);
-    p.dst = smem + (i & 1) * 2 * BUF + half * BUF + w * 16 * D * 2;
+    p.dst = smem + (i & 1) * 2 * BUF + half * BUF + (w % NP) * 16 * D * 2;
 #pragma unroll
     for (int j = 0; j < copy.N; ++j) p.off[j] = copy.off[j];
     return p;
@@ -701,7 +705,7 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
       sc[e] = seen ? sc[e] : -INFINITY;
     }
   };
-  auto softmax = [&](const Piece& kp, const Piece& vp) QTTS_PG_INLINE {
+  auto softmax = [&](const Piece& kp, const Piece& vp) QTTS_PG_INLINE {   // (vp: steps of 8 pieces)
     float bm = sc[0];
 #pragma unroll
     for (int e = 1; e < 16 * NU; ++e) bm = fmaxf(bm, sc[e]);
@@ -725,7 +729,7 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
       sum += e1;
       p[j >> 2][j & 3] = E::pack(e0, e1);
       // one copy at a time between the exponentials: issued together they hold the wave for 130 cycles each
-      constexpr int every = 8 * NU / (2 * copy.N);
+      constexpr int every = 8 * NU / (PAIR * copy.N);
       if (j % every == every - 1) {
         const int n = j / every;
         if (n < copy.N) copy.one(kp.rs, kp.dst + n * 1024, kp.off[n]);
@@ -743,8 +747,10 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
   const Entries first = entries(0);
   Entries second = entries(1);
   uint32_t has = found(first);                            // of the step computed
-  issue(piece(k_head, own(first, has), 0, 0));
-  issue(piece(v_head, own(first, has), 0, 1));
+  const int half = PAIR == 2 ? 0 : w >> 2;
+  const uint16_t* const head_a = half == 0 ? k_head : v_head;
+  issue(piece(head_a, own(first, has), 0, half));
+  if constexpr (PAIR == 2) issue(piece(v_head, own(first, has), 0, 1));
 #pragma unroll 1
   for (int i = 0; i < steps; ++i) {
     wait_vm_lds<0>();                 // this wave's copies have landed, its reads of the other buffer are done
@@ -752,7 +758,7 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
     read_k(i, 0);
     const uint32_t has_n = found(second);                 // of step i + 1
     const int page = own(second, has_n);
-    Piece kp = piece(k_head, page, i + 1, 0), vp = piece(v_head, page, i + 1, 1);
+    Piece kp = piece(head_a, page, i + 1, half), vp = PAIR == 2 ? piece(v_head, page, i + 1, 1) : kp;
     second = entries(i + 2);
     const int has_i = (int)(has >> (ks * PPB)) & ((1 << PPB) - 1);
     has = has_n;
@@ -760,7 +766,7 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
     scores(i);
     if (!whole) {
       part(kp);
-      part(vp);
+      if constexpr (PAIR == 2) part(vp);
       mask(i, has_i);
     }
     softmax(kp, vp);
@@ -772,34 +778,38 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
 
   // join the splits: M = max m_s, L = sum l_s e^(m_s - M), O = sum O_s e^(m_s - M), in key order; wave (ks, wr)
   // finishes channels ks D / NS .. of its rows
-  float* sml = reinterpret_cast<float*>(smem + 4 * BUF) + wr * NS * 2 * 32;
-  if (hf == 0) {
-    sml[(2 * ks) * 32 + c] = m;
-    sml[(2 * ks + 1) * 32 + c] = l;
-  }
-  __syncthreads();                    // every buffer is dead
-  float M = -INFINITY, L = 0.0f;
-#pragma unroll
-  for (int v = 0; v < NS; ++v) M = fmaxf(M, sml[2 * v * 32 + c]);
-#pragma unroll
-  for (int v = 0; v < NS; ++v) {
-    const float mv = sml[2 * v * 32 + c], lv = sml[(2 * v + 1) * 32 + c];
-    L += mv == -INFINITY ? lv : lv * __builtin_amdgcn_exp2f((mv - M) * SL);   // (-inf: 0, or NaN after NaN scores)
-  }
-  const float sw = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - M) * SL);
-  // [row group][split][channel block][register quad][lane][4]; O^T: column = row c, register e of block mb =
-  // channel 32 mb + 8 (e >> 2) + 4 hf + (e & 3)
+  float* sml = reinterpret_cast<float*>(smem + ROOM) + wr * NS * 2 * 32;
   float* so = reinterpret_cast<float*>(smem) + wr * NS * MB * 1024;
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f32x4 x;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[k] = o[mb][4 * e + k] * sw;
-      *reinterpret_cast<f32x4*>(so + ((ks * MB + mb) * 4 + e) * 256 + lane * 4) = x;
+  float L = l;
+  if constexpr (NS > 1) {
+    if (hf == 0) {
+      sml[(2 * ks) * 32 + c] = m;
+      sml[(2 * ks + 1) * 32 + c] = l;
     }
-  __syncthreads();
+    __syncthreads();                    // every buffer is dead
+    float M = -INFINITY;
+    L = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NS; ++v) M = fmaxf(M, sml[2 * v * 32 + c]);
+#pragma unroll
+    for (int v = 0; v < NS; ++v) {
+      const float mv = sml[2 * v * 32 + c], lv = sml[(2 * v + 1) * 32 + c];
+      L += mv == -INFINITY ? lv : lv * __builtin_amdgcn_exp2f((mv - M) * SL);   // (-inf: 0, or NaN after NaN scores)
+    }
+    const float sw = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - M) * SL);
+    // [row group][split][channel block][register quad][lane][4]; O^T: column = row c, register e of block mb =
+    // channel 32 mb + 8 (e >> 2) + 4 hf + (e & 3)
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f32x4 x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = o[mb][4 * e + k] * sw;
+        *reinterpret_cast<f32x4*>(so + ((ks * MB + mb) * 4 + e) * 256 + lane * 4) = x;
+      }
+    __syncthreads();
+  }
   const float rl = L == 0.0f ? 0.0f : 1.0f / L;
   uint16_t* op = g.out + (long long)(at.first + ti) * g.o_token + (long long)head * g.o_head + 4 * hf;
   constexpr int NQ = MB * 4 / NS;     // register quads that this wave finishes
@@ -807,10 +817,15 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
   uint32_t worst = 0u;                // largest magnitude by its bits (x - x would be contracted with the product)
 #pragma unroll
   for (int j = 0; j < NQ; ++j) {
-    const int e = ks * NQ + j;
-    y[j] = *reinterpret_cast<const f32x4*>(so + e * 256 + lane * 4);
+    if constexpr (NS > 1) {
+      const int e = ks * NQ + j;
+      y[j] = *reinterpret_cast<const f32x4*>(so + e * 256 + lane * 4);
 #pragma unroll
-    for (int v = 1; v < NS; ++v) y[j] += *reinterpret_cast<const f32x4*>(so + (v * MB * 4 + e) * 256 + lane * 4);
+      for (int v = 1; v < NS; ++v) y[j] += *reinterpret_cast<const f32x4*>(so + (v * MB * 4 + e) * 256 + lane * 4);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y[j][k] = o[j >> 2][4 * (j & 3) + k];
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       y[j][k] *= rl;
@@ -818,12 +833,13 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
     }
   }
   worst = max(worst, xlane<5>(worst));
-  // rows that are to be summed again, known to every split (their words are free again: all have read them)
-  __syncthreads();
-  if (hf == 0) sml[2 * ks * 32 + c] = __uint_as_float(worst);
-  __syncthreads();
+  if constexpr (NS > 1) {   // rows that are to be summed again, known to every split
+    __syncthreads();        // (all have read the words)
+    if (hf == 0) sml[2 * ks * 32 + c] = __uint_as_float(worst);
+    __syncthreads();
 #pragma unroll
-  for (int v = 0; v < NS; ++v) worst = max(worst, __float_as_uint(sml[2 * v * 32 + c]));
+    for (int v = 0; v < NS; ++v) worst = max(worst, __float_as_uint(sml[2 * v * 32 + c]));
+  }
   if (stored && worst < 0x7f800000u) {
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
@@ -913,11 +929,42 @@ hipError_t launch_prefill(const AttnArgs& g, hipStream_t st) {
   hipLaunchKernelGGL((prefill_kernel<E, D, NS>), dim3((unsigned)(tiles * g.hkv)), dim3(64 * PWV), 0, st, g);
   return hipGetLastError();
 }
+// Which tiles: 256 rows unsplit (NS = 1) take the fewest key steps for all the rows together, 64 rows in 4 key splits
+// the shortest chain for one tile. A launch takes the longer of the longest tile's chain and all tiles' steps over
+// the tiles that run at once (one a CU with 128 channels, two with 64), estimated with 2 to 2.5 us a tile and
+// 1.6, 2.4 and 1.6 us a step (loaded and unloaded CUs: 1.4 to 2.2). Measured us, NS = 1 : 2 : 4, of 16 / 8 heads of 128:
+// a prompt of 300 tokens 16.4 : 14.4 : 11.6, 1000 35.6 : 23.7 : 18.0, 2000 61.3 : 39.4 : 37.5, 4096 117.8 : 89.5 : 114.5,
+// 8192 278.8 : 294.8 : 366; 64 prompts of 20 to 100 25.5 : 36.1 : 40.9; 8 of 50 to 100 after 4000 104 : 57 : 44; 8192 under
+// a window of 512 77 : 81 : 107.
+template <int D>
+int prefill_splits(const AttnArgs& g, int max_len) {
+  const double each = (double)g.tokens / g.requests, slots = D == 128 ? 256 : 512;
+  int pick = 1;
+  double best = 1e30;
+  for (int ns = 1; ns <= 4; ns *= 2) {
+    const int pm = 32 * PWV / ns, step = ns == 4 ? 128 : 64 * ns;
+    const double tile = ns == 2 ? 2.5 : 2.0, cost = ns == 2 ? 2.4 : 1.6, span = (double)g.window + (double)g.sinks + (double)pm / g.group;
+    const double rows = each * g.group, n = (g.requests == 1 ? std::ceil(rows / pm) : std::max(1.0, rows / pm + 0.5)) * g.requests * g.hkv;
+    double longest = max_len, mean = std::max(max_len - each / 2, max_len / 2.0);
+    if (g.window > 0) {
+      longest = std::min(longest, span);
+      mean = std::min(mean, span);
+    }
+    const double t = std::max(tile + std::ceil(longest / step) * cost, n / slots * (tile + std::ceil(mean / step) * cost));
+    if (t < best) {
+      best = t;
+      pick = ns;
+    }
+  }
+  return pick;
+}
 template <class E, int D>
-hipError_t prefill_split(const AttnArgs& g, hipStream_t st) {
-  static const char* e = getenv("QNS");
-  if (e && e[0] == '4') return launch_prefill<E, D, 4>(g, st);
-  return launch_prefill<E, D, 2>(g, st);
+hipError_t launch_prefill_any(const AttnArgs& g, int max_len, hipStream_t st) {
+  switch (prefill_splits<D>(g, max_len)) {
+    case 1: return launch_prefill<E, D, 1>(g, st);
+    case 2: return launch_prefill<E, D, 2>(g, st);
+    default: return launch_prefill<E, D, 4>(g, st);
+  }
 }
 
 }  // namespace pg
@@ -975,17 +1022,19 @@ hipError_t qtts_paged_attention_prefill(const QttsPagedCache* cache, int n_reque
                                         const void* q, long long q_token_stride, long long q_head_stride, void* out,
                                         long long out_token_stride, long long out_head_stride, const int* block_table,
                                         int table_width, long long table_stride, const int* kv_lens, const int* cu_tokens,
-                                        float scale, int window, int sinks, hipStream_t stream) {
+                                        int max_len, float scale, int window, int sinks, hipStream_t stream) {
   if (!attn_ok(cache, n_tokens, num_q_heads, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
-               block_table, table_width, table_stride, kv_lens, n_requests, scale, window, sinks) || cu_tokens == nullptr)
+               block_table, table_width, table_stride, kv_lens, n_requests, scale, window, sinks) || cu_tokens == nullptr || max_len < 1)
     return hipErrorInvalidValue;
   if (n_tokens == 0) return hipSuccess;
   AttnArgs g = attn_args(cache, num_q_heads, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
                          block_table, table_width, table_stride, kv_lens, n_requests, scale, window, sinks);
   g.cu = cu_tokens;
   g.tokens = n_tokens;
-  if (cache->dtype == QTTS_BF16) return cache->head_dim == 128 ? prefill_split<Bf16, 128>(g, stream) : prefill_split<Bf16, 64>(g, stream);
-  return cache->head_dim == 128 ? prefill_split<F16, 128>(g, stream) : prefill_split<F16, 64>(g, stream);
+  const int most = (int)std::min<long long>(max_len, (long long)table_width * cache->page_size);
+  if (cache->dtype == QTTS_BF16)
+    return cache->head_dim == 128 ? launch_prefill_any<Bf16, 128>(g, most, stream) : launch_prefill_any<Bf16, 64>(g, most, stream);
+  return cache->head_dim == 128 ? launch_prefill_any<F16, 128>(g, most, stream) : launch_prefill_any<F16, 64>(g, most, stream);
 }
 
 }  // extern "C"
