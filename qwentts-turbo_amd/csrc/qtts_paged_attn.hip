@@ -97,15 +97,19 @@ struct PieceCopy {
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] = seen(key0 + RPI * i + lane / CPR) ? off[i] : 0x7fffff00;
   }
+  // ONCE: the bytes are read once and need no place in the caches
+  template <bool ONCE = false>
   __device__ __forceinline__ static void one(__amdgpu_buffer_rsrc_t rs, char* dst, int o) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lvoid_t*)dst, 16, o, 0, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lvoid_t*)dst, 16, o, 0, 0, ONCE ? 2 : 0);
   }
 };
 
 // ---- decode --------------------------------------------------------------------------------
-// One workgroup of 4 waves per (request, KV head, up to 16 of its query heads, part of its keys). Bound by
-// reading K and V: every wave streams its own 32-key blocks (blocks w, w + 4, .. of the unit) through two
-// LDS buffers of its own, so the loop has no barrier, and 64 KB or more a CU are in flight.
+// One workgroup of W waves per (request, KV head, up to 16 of its query heads, part of its keys: a unit). Bound by
+// reading K and V: every wave streams its own 32-key blocks (blocks w, w + W, .. of the unit) through LDS rows of its
+// own, so the loop has no barrier. The next block's K goes out as soon as this one's scores are taken, its V after
+// the products, so that 16 KB a wave (128 channels) are in flight nearly always; two workgroups of 4 waves fit a CU,
+// and one's beginning and end run under the other's stream.
 //   S^T = K Q^T on MFMA 16x16x32 (A: 16 keys x 32 channels from LDS, B: Q^T in registers): lane (g, c) holds
 //     head c's scores of keys 4 g + r and 16 + 4 g + r, r < 4; the max over a head's keys is in-lane and two
 //     exchanges.
@@ -113,10 +117,9 @@ struct PieceCopy {
 //     16 + 4 g + j - 4 above), V^T comes through LDS transpose reads of 4 keys each. P goes in as two 16-bit
 //     numbers, the rounded value and the rounded rest, so that its rounding is that of 16 bits or more: the
 //     matrix units are idle otherwise.
-// The heads of a group share every K and V byte; a group over 16 is several workgroups. The 4 waves join
-// through LDS, the units of a request through part / part_ml and decode_join_kernel, both in key order, so
-// results do not depend on timing. A request of one unit writes its output here.
-constexpr int DW = 4;                 // waves
+// The heads of a group share every K and V byte; a group over 16 is several workgroups. The waves join through
+// LDS, the units of a request through part / part_ml and decode_join_kernel, both in key order, so results do not
+// depend on timing. A request of one unit writes its output here.
 constexpr int DKB = 32;               // keys of a block
 
 // The transpose reads of an MFMA step: 4 keys at LDS addresses a[..] + A and 4 more at b[..] + B, of each channel
@@ -152,12 +155,12 @@ __device__ __forceinline__ void tr_read16(const uint32_t (&a)[4], const uint32_t
       : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]), "i"(A), "i"(B), "i"(A + S), "i"(B + S)
       : "memory");
 }
-template <class E, int D>
-__global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
+template <class E, int D, int W>
+__global__ void __launch_bounds__(64 * W, 2) decode_kernel(const AttnArgs g) {
   constexpr int BLK = DKB * D * 2;               // bytes of a K or V block
   constexpr int MB = D / 16, KS = D / 32;        // 16-channel blocks of O^T, MFMA steps of a score
-  constexpr int NL = 2 * DKB * D * 2 / 1024;     // DMA instructions of a block
-  __shared__ __attribute__((aligned(1024))) char smem[DW * 4 * BLK];   // (K, V) x 2 buffers a wave
+  constexpr int NL = BLK / 1024;                 // DMA instructions of a K or V block
+  __shared__ __attribute__((aligned(1024))) char smem[W * 2 * BLK + (2 * W + 2) * 16 * 4];   // (K, V) a wave; (m, l) of the join
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int c = lane & 15, gr = lane >> 4;
   int id = blockIdx.x;
@@ -174,7 +177,7 @@ __global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
   const int units = max(1, (bl.n + per - 1) / per);
   if (unit >= units) return;
   const int t1 = min(bl.n, (unit + 1) * per), t0 = unit * per + w;
-  const int nt = t0 < t1 ? (t1 - t0 + DW - 1) / DW : 0;   // this wave's blocks
+  const int nt = t0 < t1 ? (t1 - t0 + W - 1) / W : 0;   // this wave's blocks
 
   // Q^T: head c, channels 32 s + 8 gr ..
   u32x4 q[KS];
@@ -182,40 +185,53 @@ __global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
 #pragma unroll
   for (int s = 0; s < KS; ++s) q[s] = ldw(qp + 32 * s);
 
-  char* const buf = smem + w * 4 * BLK;
+  char* const buf = smem + w * 2 * BLK;
   const int* row = g.table + (long long)b * g.table_stride;
-  auto block_at = [&](int i) QTTS_PG_INLINE { const int t = t0 + DW * i; return t < bl.ns ? t : t + bl.skip; };
-  // pages of 32 of the wave's blocks, one 16-key piece a lane (-1: none)
-  auto pages_from = [&](int i0) QTTS_PG_INLINE {
-    const int key = block_at(i0 + (lane >> 1)) * DKB + 16 * (lane & 1);
-    int p = -1;
-    if (i0 + (lane >> 1) < nt && key < len) p = *gmem(row + (key >> g.pages.shift));
-    return (unsigned)p < (unsigned)g.pages.num_pages ? p : -1;
+  auto key_of = [&](int i) QTTS_PG_INLINE { const int t = t0 + W * i; return (t < bl.ns ? t : t + bl.skip) * DKB; };
+  // the table entries of a block's two pieces, piece lane & 1 a lane, loaded a block before they are used
+  struct Entries {
+    int e;
+    uint32_t in;                                 // pieces that have keys, as bits
   };
-  int held = pages_from(0), next_held = 0;
-  uint64_t has = __builtin_amdgcn_ballot_w64(held >= 0);      // of block i: bits 2 (i & 31), + 1
+  auto entries = [&](int i) QTTS_PG_INLINE {
+    const int key = key_of(i) + 16 * (lane & 1);
+    const bool in = (i < nt) & (key < len);
+    return Entries{*gmem(row + (in ? key >> g.pages.shift : 0)), (uint32_t)__builtin_amdgcn_ballot_w64(in) & 3u};
+  };
+  // a block as it is copied: pages of its pieces (bits of `has`), and the lane's offsets where only a part is seen
   const PieceCopy<D> copy(g.pages.slot_stride, lane);
   const uint16_t* const k_head = g.pages.k + (long long)kvh * g.pages.head_stride;
   const uint16_t* const v_head = g.pages.v + (long long)kvh * g.pages.head_stride;
-  auto issue = [&](int i) QTTS_PG_INLINE {
-    const int kb = block_at(i);
-    char* dst = buf + (i & 1) * 2 * BLK;
+  struct Block {
+    int key0, page[2];
+    uint32_t has;
+    bool whole;
+  };
+  auto block = [&](const Entries& x, int i) QTTS_PG_INLINE {
+    Block r;
+    r.key0 = key_of(i);
+    r.has = (uint32_t)__builtin_amdgcn_ballot_w64((unsigned)x.e < (unsigned)g.pages.num_pages) & x.in;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int page = __builtin_amdgcn_readlane(held, 2 * (i & 31) + u);
-      const int k0 = kb * DKB + 16 * u;
-      const bool whole = page >= 0 && k0 + 16 <= len && (k0 >= lo || k0 + 16 <= g.sinks);
-      auto seen = [&](int key) QTTS_PG_INLINE { return (page >= 0) & (key < len) & ((key >= lo) | (key < g.sinks)); };
-      const auto kr = copy.piece(k_head, g.pages, max(page, 0), k0), vr = copy.piece(v_head, g.pages, max(page, 0), k0);
+      const int page = __builtin_amdgcn_readlane(x.e, u);
+      r.page[u] = (r.has >> u) & 1 ? page : 0;
+    }
+    r.whole = (r.has == 3u) & (r.key0 + DKB <= len) & ((r.key0 >= lo) | (r.key0 + DKB <= g.sinks));
+    return r;
+  };
+  auto sees = [&](const Block& r, int key, int u) QTTS_PG_INLINE {
+    return (((r.has >> u) & 1) != 0) & (key < len) & ((key >= lo) | (key < g.sinks));
+  };
+  auto issue = [&](const Block& r, const uint16_t* head, char* dst) QTTS_PG_INLINE {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const auto rs = copy.piece(head, g.pages, r.page[u], r.key0 + 16 * u);
       int off[copy.N];
 #pragma unroll
       for (int j = 0; j < copy.N; ++j) off[j] = copy.off[j];
-      if (!whole) copy.some(k0, lane, off, seen);
+      if (!r.whole) copy.some(r.key0 + 16 * u, lane, off, [&](int key) QTTS_PG_INLINE { return sees(r, key, u); });
 #pragma unroll
-      for (int j = 0; j < copy.N; ++j) {
-        copy.one(kr, dst + u * 16 * D * 2 + j * 1024, off[j]);
-        copy.one(vr, dst + BLK + u * 16 * D * 2 + j * 1024, off[j]);
-      }
+      for (int j = 0; j < copy.N; ++j) copy.template one<true>(rs, dst + u * 16 * D * 2 + j * 1024, off[j]);
     }
   };
 
@@ -226,104 +242,105 @@ __global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
   for (int mb = 0; mb < MB; ++mb) o[mb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   // transpose reads of V: row 4 gr + (c >> 2), chunk 2 mb + ((c & 3) >> 1), 8 bytes at 8 (c & 1)
   const int vrow = 4 * gr + (c >> 2);
-  uint32_t vaddr[4];
+  uint32_t va[4];
 #pragma unroll
   for (int mb = 0; mb < 4; ++mb)
-    vaddr[mb] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)buf + BLK + vrow * D * 2 +
-                ((2 * mb + ((c & 3) >> 1)) ^ swz<D>(vrow)) * 16 + 8 * (c & 1);
+    va[mb] = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)buf + BLK + vrow * D * 2 +
+             ((2 * mb + ((c & 3) >> 1)) ^ swz<D>(vrow)) * 16 + 8 * (c & 1);
 
-  if (nt > 0) issue(0);
+  if (nt > 0) {
+    Entries ahead = entries(1);
+    Block now = block(entries(0), 0);
+    issue(now, k_head, buf);
+    issue(now, v_head, buf + BLK);
 #pragma unroll 1
-  for (int i = 0; i < nt; ++i) {
-    const uint64_t has_i = has >> (2 * (i & 31));
-    if (i + 1 < nt) {
-      if (((i + 1) & 31) == 0) {
-        held = pages_from(i + 1);
-        has = __builtin_amdgcn_ballot_w64(held >= 0);
-      }
-      issue(i + 1);
-      wait_vm_lds<NL>();
-    } else {
-      wait_vm_lds<0>();
-    }
-    asm volatile("" ::: "memory");
-    const char* K = buf + (i & 1) * 2 * BLK;
-    f32x4 sc[2];
+    for (int i = 0; i < nt; ++i) {
+      const Block next = block(ahead, i + 1);
+      ahead = entries(i + 2);
+      wait_vm_lds<NL + 1>();                     // K is here: V's copies and the entries may be under way
+      asm volatile("" ::: "memory");
+      f32x4 sc[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      sc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int u = 0; u < 2; ++u) {
+        sc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const u32x4 k = *reinterpret_cast<const u32x4*>(K + (16 * u + c) * D * 2 + ((4 * s + gr) ^ swz<D>(c)) * 16);
-        sc[u] = E::mma16(k, q[s], sc[u]);
+        for (int s = 0; s < KS; ++s) {
+          const u32x4 k = *reinterpret_cast<const u32x4*>(buf + (16 * u + c) * D * 2 + ((4 * s + gr) ^ swz<D>(c)) * 16);
+          sc[u] = E::mma16(k, q[s], sc[u]);
+        }
       }
-    }
-    const int key0 = block_at(i) * DKB;
-    if (!((has_i & 3) == 3 && key0 + DKB <= len && (key0 >= lo || key0 + DKB <= g.sinks))) {
+      asm volatile("" : "+v"(sc[0]), "+v"(sc[1]) :: "memory");   // K has been read
+      if (i + 1 < nt) issue(next, k_head, buf);
+      if (!now.whole) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sc[u][r] = sees(now, now.key0 + 16 * u + 4 * gr + r, u) ? sc[u][r] : -INFINITY;
+      }
+      float bm = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                       fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+      bm = fmaxf(bm, xlane_f<4>(bm));
+      bm = fmaxf(bm, xlane_f<5>(bm));
+      if (__builtin_amdgcn_ballot_w64(bm > m) != 0ull) {
+        const float mn = fmaxf(m, bm);
+        const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * SL);
+        l *= al;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[mb][r] *= al;
+        m = mn;
+      }
+      const float nm = m == -INFINITY ? 0.0f : -m * SL;
+      u32x4 ph, pl;
+      float sum = 0.0f;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = key0 + 16 * u + 4 * gr + r;
-          const bool seen = (((has_i >> u) & 1) != 0) & (key < len) & ((key >= lo) | (key < g.sinks));
-          sc[u][r] = seen ? sc[u][r] : -INFINITY;
+        for (int h = 0; h < 2; ++h) {
+          const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[u][2 * h], SL, nm)), e1 = __builtin_amdgcn_exp2f(fmaf(sc[u][2 * h + 1], SL, nm));
+          sum += e0 + e1;
+          const uint32_t p = E::pack(e0, e1);
+          ph[2 * u + h] = p;
+          pl[2 * u + h] = E::pack(e0 - E::lo(p), e1 - E::hi(p));
         }
-    }
-    float bm = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                     fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-    bm = fmaxf(bm, xlane_f<4>(bm));
-    bm = fmaxf(bm, xlane_f<5>(bm));
-    if (__builtin_amdgcn_ballot_w64(bm > m) != 0ull) {
-      const float mn = fmaxf(m, bm);
-      const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * SL);
-      l *= al;
+      l += sum;
+      if (i + 1 < nt) wait_vm_lds<NL + 1>();     // V is here: the next K's copies and the entries may be under way
+      else wait_vm_lds<1>();
+      auto pv = [&](int half, const u32x2 (&a)[4], const u32x2 (&bq)[4]) QTTS_PG_INLINE {
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[mb][r] *= al;
-      m = mn;
-    }
-    const float nm = m == -INFINITY ? 0.0f : -m * SL;
-    u32x4 ph, pl;
-    float sum = 0.0f;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[u][2 * h], SL, nm)), e1 = __builtin_amdgcn_exp2f(fmaf(sc[u][2 * h + 1], SL, nm));
-        sum += e0 + e1;
-        const uint32_t p = E::pack(e0, e1);
-        ph[2 * u + h] = p;
-        pl[2 * u + h] = E::pack(e0 - E::lo(p), e1 - E::hi(p));
-      }
-    l += sum;
-    uint32_t va[4];
-#pragma unroll
-    for (int mb = 0; mb < 4; ++mb) va[mb] = vaddr[mb] + (i & 1) * 2 * BLK;
-    auto pv = [&](int half, const u32x2 (&a)[4], const u32x2 (&bq)[4]) QTTS_PG_INLINE {
-#pragma unroll
-      for (int mb = 0; mb < 4; ++mb) {
-        const u32x4 v = {a[mb][0], a[mb][1], bq[mb][0], bq[mb][1]};
-        o[4 * half + mb] = E::mma16(v, ph, o[4 * half + mb]);
-        o[4 * half + mb] = E::mma16(v, pl, o[4 * half + mb]);
-      }
-    };
-    u32x2 a[4], bq[4];
-    tr_read8<0, 16 * D * 2>(va, va, a, bq);
-    pv(0, a, bq);
-    if constexpr (D == 128) {
-#pragma unroll
-      for (int mb = 0; mb < 4; ++mb) va[mb] ^= 128;   // channels 64 ..
+        for (int mb = 0; mb < 4; ++mb) {
+          const u32x4 v = {a[mb][0], a[mb][1], bq[mb][0], bq[mb][1]};
+          o[4 * half + mb] = E::mma16(v, ph, o[4 * half + mb]);
+          o[4 * half + mb] = E::mma16(v, pl, o[4 * half + mb]);
+        }
+      };
+      u32x2 a[4], bq[4];
       tr_read8<0, 16 * D * 2>(va, va, a, bq);
-      pv(1, a, bq);
+      if constexpr (D == 128) {
+        uint32_t vb[4];
+        u32x2 a2[4], bq2[4];
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb) vb[mb] = va[mb] ^ 128;   // channels 64 ..
+        tr_read8<0, 16 * D * 2>(vb, vb, a2, bq2);
+        if (i + 1 < nt) issue(next, v_head, buf + BLK);
+        pv(0, a, bq);
+        pv(1, a2, bq2);
+      } else {
+        if (i + 1 < nt) issue(next, v_head, buf + BLK);
+        pv(0, a, bq);
+      }
+      now = next;
     }
   }
   l += xlane_f<4>(l);
   l += xlane_f<5>(l);
 
   // join the waves: M = max m_w, L = sum l_w e^(m_w - M), O = sum O_w e^(m_w - M)
+  static_assert(D * 16 * 4 <= 2 * BLK, "the join's sums");
+  wait_vm_lds<0>();
   __syncthreads();                               // every buffer is dead
-  float* sml = reinterpret_cast<float*>(smem + DW * D * 16 * 4);
+  float* sml = reinterpret_cast<float*>(smem + W * 2 * BLK);
   if (gr == 0) {
     sml[(2 * w) * 16 + c] = m;
     sml[(2 * w + 1) * 16 + c] = l;
@@ -331,9 +348,9 @@ __global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
   __syncthreads();
   float M = -INFINITY, L = 0.0f;
 #pragma unroll
-  for (int v = 0; v < DW; ++v) M = fmaxf(M, sml[2 * v * 16 + c]);
+  for (int v = 0; v < W; ++v) M = fmaxf(M, sml[2 * v * 16 + c]);
 #pragma unroll
-  for (int v = 0; v < DW; ++v) {
+  for (int v = 0; v < W; ++v) {
     const float mv = sml[2 * v * 16 + c];
     L += mv == -INFINITY ? sml[(2 * v + 1) * 16 + c] : sml[(2 * v + 1) * 16 + c] * __builtin_amdgcn_exp2f((mv - M) * SL);
   }
@@ -347,18 +364,18 @@ __global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
     *reinterpret_cast<f32x4*>(so + (w * 16 + c) * D + 16 * mb + 4 * gr) = x;
   }
   if (w == 0 && gr == 0) {
-    sml[DW * 2 * 16 + c] = M;
-    sml[DW * 2 * 16 + 16 + c] = L;
+    sml[W * 2 * 16 + c] = M;
+    sml[W * 2 * 16 + 16 + c] = L;
   }
   __syncthreads();
   const bool whole = units == 1;
-  for (int e = threadIdx.x; e < nh * D / 4; e += 64 * DW) {
+  for (int e = threadIdx.x; e < nh * D / 4; e += 64 * W) {
     const int h = e / (D / 4), d = 4 * (e % (D / 4));
     f32x4 x = *reinterpret_cast<const f32x4*>(so + h * D + d);
 #pragma unroll
-    for (int v = 1; v < DW; ++v) x += *reinterpret_cast<const f32x4*>(so + (v * 16 + h) * D + d);
+    for (int v = 1; v < W; ++v) x += *reinterpret_cast<const f32x4*>(so + (v * 16 + h) * D + d);
     if (whole) {
-      const float Lh = sml[DW * 2 * 16 + 16 + h];
+      const float Lh = sml[W * 2 * 16 + 16 + h];
       const float rl = Lh == 0.0f ? 0.0f : 1.0f / Lh;
       u32x2 p;
       p[0] = E::pack(x[0] * rl, x[1] * rl);
@@ -368,45 +385,75 @@ __global__ void __launch_bounds__(64 * DW) decode_kernel(const AttnArgs g) {
       const long long at = ((long long)b * g.hq + head0 + h) * g.splits + unit;
       *reinterpret_cast<f32x4*>(g.part + at * D + d) = x;
       if (d == 0) {
-        g.part_ml[2 * at] = sml[DW * 2 * 16 + h];
-        g.part_ml[2 * at + 1] = sml[DW * 2 * 16 + 16 + h];
+        g.part_ml[2 * at] = sml[W * 2 * 16 + h];
+        g.part_ml[2 * at + 1] = sml[W * 2 * 16 + 16 + h];
       }
     }
   }
 }
 
-// The units of a request's head joined in key order: one wave per (request, query head).
+// The units of a request's head joined: one workgroup per (request, query head), its D / 4 lanes a unit taking 4
+// channels each and its groups of lanes units u, u + groups, ..; the groups' sums add through LDS in order. Loads do
+// not wait for the request's length (what a unit past its last has in its place is passed over), so the chain is one
+// read, not three.
 template <class E, int D>
 __global__ void __launch_bounds__(256) decode_join_kernel(const AttnArgs g) {
-  constexpr int DL = D / 64;
-  const int lane = threadIdx.x & 63;
-  const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (id >= (long long)g.requests * g.hq) return;
-  const int b = (int)(id / g.hq), h = (int)(id % g.hq);
+  constexpr int LU = D / 4, GR = 256 / LU, AT = 4;   // lanes a unit, groups, units of a group read at once
+  __shared__ float sums[GR][D + 4];
+  const int t = threadIdx.x, gq = t / LU, d = 4 * (t % LU);
+  const int b = blockIdx.x / g.hq, h = blockIdx.x % g.hq;
+  const long long id = blockIdx.x;
+  const float* ml = g.part_ml + 2 * id * g.splits;
+  const float* po = g.part + id * g.splits * D + d;
+  f32x4 x[AT];
+  float mu[AT], lu[AT];
+  auto read = [&](int u0) QTTS_PG_INLINE {
+#pragma unroll
+    for (int k = 0; k < AT; ++k) {
+      const int u = min(u0 + gq + GR * k, g.splits - 1);
+      x[k] = *reinterpret_cast<const f32x4*>(po + (long long)u * D);
+      mu[k] = ml[2 * u];
+      lu[k] = ml[2 * u + 1];
+    }
+  };
+  read(0);
   const int len = request_len(g, b);
   const Blocks bl = blocks_of<DKB>(g.window > 0 ? max(len - g.window, 0) : 0, len, g.sinks);
   const int per = max(g.blocks, (bl.n + g.splits - 1) / g.splits), units = (bl.n + per - 1) / per;
   if (units <= 1) return;
-  const float* ml = g.part_ml + 2 * id * g.splits;
-  const float* po = g.part + id * g.splits * D + DL * lane;
-  float M = -INFINITY;
-  for (int u = lane; u < units; u += 64) M = fmaxf(M, ml[2 * u]);
-  M = group_max<64>(M);
-  float L = 0.0f, x[DL] = {};
-#pragma unroll 4
-  for (int u = 0; u < units; ++u) {
-    const float mu = ml[2 * u], wu = mu == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((mu - M) * g.scale_log2);
-    L += ml[2 * u + 1] * wu;
+  float M = -INFINITY, L = 0.0f;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto take = [&](float m2, float l2, const f32x4& x2) QTTS_PG_INLINE {
+    const float mn = fmaxf(M, m2);
+    const float a = M == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((M - mn) * g.scale_log2);   // (-inf: sums are 0, or NaN)
+    const float e = m2 == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m2 - mn) * g.scale_log2);
+    L = L * a + l2 * e;
 #pragma unroll
-    for (int i = 0; i < DL; ++i) x[i] += po[(long long)u * D + i] * wu;
+    for (int i = 0; i < 4; ++i) o[i] = o[i] * a + x2[i] * e;
+    M = mn;
+  };
+  for (int u0 = 0;;) {
+#pragma unroll
+    for (int k = 0; k < AT; ++k)
+      if (u0 + gq + GR * k < units) take(mu[k], lu[k], x[k]);
+    u0 += GR * AT;
+    if (u0 >= units) break;
+    read(u0);
   }
+  *reinterpret_cast<f32x4*>(&sums[gq][d]) = o;
+  if (d == 0) {
+    sums[gq][D] = M;
+    sums[gq][D + 1] = L;
+  }
+  __syncthreads();
+  if (gq != 0) return;
+#pragma unroll
+  for (int k = 1; k < GR; ++k) take(sums[k][D], sums[k][D + 1], *reinterpret_cast<const f32x4*>(&sums[k][d]));
   const float rl = L == 0.0f ? 0.0f : 1.0f / L;
-  uint16_t* op = g.out + (long long)b * g.o_token + (long long)h * g.o_head + DL * lane;
-  if constexpr (DL == 2) {
-    *reinterpret_cast<uint32_t*>(op) = E::pack(x[0] * rl, x[1] * rl);
-  } else {
-    *op = (uint16_t)E::pack(x[0] * rl, 0.0f);
-  }
+  u32x2 p;
+  p[0] = E::pack(o[0] * rl, o[1] * rl);
+  p[1] = E::pack(o[2] * rl, o[3] * rl);
+  *reinterpret_cast<u32x2*>(g.out + (long long)b * g.o_token + (long long)h * g.o_head + d) = p;
 }
 
 // ---- prefill -------------------------------------------------------------------------------
@@ -896,28 +943,36 @@ AttnArgs attn_args(const QttsPagedCache* cache, int hq, const void* q, long long
   return g;
 }
 
-// How decode splits a request: units of at least 4 blocks (one a wave), as many as give every CU work.
+// How decode splits requests into units. Pairs of a request and a KV head that fill the GPU by themselves (128 on) are
+// split only where they are long: a second launch joins the units, and short units are mostly their own beginning
+// and end (us, unsplit against units of 512 keys: 200 requests of 100 to 700 keys 59.5 : 88.9, 64 of 50 to 300
+// 13.3 : 22.7 (256 keys); 24 under a window of 1024 21.6 : 26.5), but 64 ragged ones up to 4090 keys leave a shorter last
+// round (101.8 : 108.8, 16 up to 4000 31.0 : 33.5). Fewer pairs are split down to 256 keys a unit, until there
+// are 512 units (one request of 700 keys 9.8 : 10.1 unsplit, of 2000 10.7 : 21.7, of 60000 in 512 units 46.7, in 1024
+// 49.8).
 struct Split {
-  int splits, blocks;
+  int splits, blocks;      // most units, blocks a unit
+  bool wide;               // 8 waves a workgroup: for unsplit pairs that leave a CU one workgroup
 };
 Split decode_split(int requests, int hkv, int group, int width, int page_size, int max_len, int window, int sinks) {
   long long keys = std::min<long long>((long long)width * page_size, max_len);
   if (window > 0) keys = std::min<long long>(keys, (long long)window + std::min<long long>(sinks, keys) + 2 * DKB);
   const long long blocks = std::max<long long>(1, (keys + DKB - 1) / DKB);
   const long long pairs = (long long)requests * hkv * ((group + 15) / 16);
-  const long long want = std::max<long long>(1, 1024 / pairs);
-  long long per = std::max<long long>(16, (blocks + want - 1) / want);
-  per = (per + DW - 1) / DW * DW;
-  const long long splits = (blocks + per - 1) / per;
-  return Split{(int)splits, (int)per};
+  if (pairs >= 128 && blocks < 64) return Split{1, (int)blocks, pairs <= 256};
+  const long long units = pairs >= 128 ? 4096 : 512, least = pairs > 256 ? 16 : 8;
+  long long per = std::max(least, (blocks * pairs + units - 1) / units);
+  per = std::min((per + 3) / 4 * 4, blocks);
+  return Split{(int)((blocks + per - 1) / per), (int)per, false};
 }
 
 template <class E, int D>
-void launch_decode(const AttnArgs& g, hipStream_t st) {
+void launch_decode(const AttnArgs& g, bool wide, hipStream_t st) {
   const int tiles = (g.group + 15) / 16;
-  hipLaunchKernelGGL((decode_kernel<E, D>), dim3((unsigned)((long long)g.requests * g.hkv * tiles * g.splits)), dim3(64 * DW), 0, st, g);
-  if (g.splits > 1)
-    hipLaunchKernelGGL((decode_join_kernel<E, D>), dim3((unsigned)(((long long)g.requests * g.hq + 3) / 4)), dim3(256), 0, st, g);
+  const dim3 grid((unsigned)((long long)g.requests * g.hkv * tiles * g.splits));
+  if (wide) hipLaunchKernelGGL((decode_kernel<E, D, 8>), grid, dim3(512), 0, st, g);
+  else hipLaunchKernelGGL((decode_kernel<E, D, 4>), grid, dim3(256), 0, st, g);
+  if (g.splits > 1) hipLaunchKernelGGL((decode_join_kernel<E, D>), dim3((unsigned)(g.requests * g.hq)), dim3(256), 0, st, g);
 }
 
 template <class E, int D, int NS>
@@ -1009,11 +1064,11 @@ hipError_t qtts_paged_attention_decode(const QttsPagedCache* cache, int n_reques
   }
   if ((long long)n_requests * g.hkv * ((g.group + 15) / 16) * g.splits > INT_MAX) return hipErrorInvalidValue;
   if (cache->dtype == QTTS_BF16) {
-    if (cache->head_dim == 128) launch_decode<Bf16, 128>(g, stream);
-    else launch_decode<Bf16, 64>(g, stream);
+    if (cache->head_dim == 128) launch_decode<Bf16, 128>(g, s.wide, stream);
+    else launch_decode<Bf16, 64>(g, s.wide, stream);
   } else {
-    if (cache->head_dim == 128) launch_decode<F16, 128>(g, stream);
-    else launch_decode<F16, 64>(g, stream);
+    if (cache->head_dim == 128) launch_decode<F16, 128>(g, s.wide, stream);
+    else launch_decode<F16, 64>(g, s.wide, stream);
   }
   return hipGetLastError();
 }
