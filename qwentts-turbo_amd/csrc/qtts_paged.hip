@@ -18,31 +18,40 @@ namespace pg {
 //   and a request that finds too few ends the giving (those behind it do not overtake it)
 //   table[b][ceil(L_b / P) + j] = free_pages[F - 1 - (need_0 + .. + need_{b-1}) - j]
 //   token i of b: position L_b + i, slot table[b][(L_b + i) / P] P + (L_b + i) % P, or -1 if not granted
-// One workgroup: two prefix sums over the requests, 1024 at a time, then the new pages and the tokens as
-// flat lists, each element finding its request by a search in LDS. It is bound by latency: the chain is
-// lengths -> sums -> free pages -> slots.
+// One workgroup: the prefix sums of tokens and pages over the requests, NT at a time, then the new pages and the
+// tokens as flat lists, each element finding its request by a search in LDS. It is bound by latency: the chain is
+// lengths -> sums -> free pages -> slots; 256 threads for up to 256 requests, whose sums cross 4 waves and not 16.
 constexpr int PT = 1024;
 
-// Inclusive prefix sum over the workgroup; *total receives the sum. `part`: PT / 64 words of LDS.
-__device__ __forceinline__ long long block_scan(long long x, long long* part, long long* total) {
+// Inclusive prefix sums of N values over the workgroup of NT threads; total[] receives the sums. `part`: N * NT / 64
+// words of LDS.
+template <int NT, int N>
+__device__ __forceinline__ void block_scan(long long (&x)[N], long long* part, long long (&total)[N]) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long long y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();                      // the words' readers of an earlier scan are done
-  if (lane == 63) part[w] = x;
-  __syncthreads();
-  long long before = 0, all = 0;
+  for (int o = 1; o < 64; o <<= 1)
 #pragma unroll
-  for (int i = 0; i < PT / 64; ++i) {
-    const long long p = part[i];
-    before += i < w ? p : 0;
-    all += p;
+    for (int k = 0; k < N; ++k) {
+      const long long y = __shfl_up(x[k], o, 64);
+      if (lane >= o) x[k] += y;
+    }
+  __syncthreads();                      // the words' readers of an earlier scan are done
+  if (lane == 63)
+#pragma unroll
+    for (int k = 0; k < N; ++k) part[k * (NT / 64) + w] = x[k];
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    long long before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) {
+      const long long p = part[k * (NT / 64) + i];
+      before += i < w ? p : 0;
+      all += p;
+    }
+    total[k] = all;
+    x[k] += before;
   }
-  *total = all;
-  return x + before;
 }
 
 // The first i < n with cum[i] > x (cum non-decreasing, x below its last entry).
@@ -80,28 +89,39 @@ __device__ __forceinline__ int slot_of(int page, int pos, int shift) {
   return page < 0 || s > INT_MAX ? -1 : (int)s;
 }
 
-__global__ void __launch_bounds__(PT) plan_kernel(const PlanArgs g) {
-  __shared__ long long part[PT / 64];
-  __shared__ long long s_taken[PT];   // pages asked up to and with the request
-  __shared__ int s_cu[PT];            // tokens up to and with the request
-  __shared__ int s_len[PT], s_have[PT];   // s_have: -1 where the request is refused
+template <int NT>
+__global__ void __launch_bounds__(NT) plan_kernel(const PlanArgs g) {
+  __shared__ long long part[2 * NT / 64];
+  __shared__ long long s_taken[NT];   // pages asked up to and with the request
+  __shared__ int s_cu[NT];            // tokens up to and with the request
+  __shared__ int s_len[NT], s_have[NT];   // s_have: -1 where the request is refused
+  __shared__ long long s_given;
   const int t = threadIdx.x;
   const long long page = 1ll << g.shift, keys = (long long)g.width << g.shift;
   const long long free_n = min(max(*g.free_count, 0), g.capacity);
-  long long carry_n = 0, carry_taken = 0, given = 0;
-  if (t == 0) g.cu[0] = 0;
-  for (int base = 0; base < g.n; base += PT) {
+  long long carry_n = 0, carry_taken = 0;
+  if (t == 0) {
+    g.cu[0] = 0;
+    s_given = 0;
+  }
+  for (int base = 0; base < g.n; base += NT) {
     const int b = base + t;
     const bool in = b < g.n;
     const long long add = in ? max(g.new_tokens[b], 0) : 0, len = in ? max(g.lengths[b], 0) : 0;
-    long long sum_n, sum_taken, sum_given;
-    const long long end = carry_n + block_scan(add, part, &sum_n);
-    const bool room = end <= g.total, full = len + add > keys, fits = in && room && !full;
-    const long long have = (len + page - 1) >> g.shift;
-    const long long need = fits ? ((len + add + page - 1) >> g.shift) - have : 0;
-    const long long taken = carry_taken + block_scan(need, part, &sum_taken);
+    const bool full = len + add > keys;
+    const long long have = (len + page - 1) >> g.shift, want = ((len + add + page - 1) >> g.shift) - have;
+    long long x[2] = {add, full ? 0 : want}, sum[2];
+    block_scan<NT>(x, part, sum);
+    const long long end = carry_n + x[0];
+    const bool room = end <= g.total, fits = in && room && !full;
+    if (carry_n + sum[0] > g.total) {     // tokens past the arrays: their pages are not asked for
+      long long y[1] = {fits ? want : 0}, ysum[1];
+      block_scan<NT>(y, part, ysum);
+      x[1] = y[0];
+      sum[1] = ysum[0];
+    }
+    const long long need = fits ? want : 0, taken = carry_taken + x[1], sum_n = sum[0], sum_taken = sum[1];
     const bool ok = fits && (need == 0 || taken <= free_n);
-    block_scan(ok ? need : 0, part, &sum_given);
     s_taken[t] = taken;
     s_cu[t] = (int)min(end, (long long)INT_MAX);
     s_len[t] = (int)len;
@@ -113,9 +133,11 @@ __global__ void __launch_bounds__(PT) plan_kernel(const PlanArgs g) {
       g.status[b] = !room ? 3 : (full ? 2 : (ok ? 0 : 1));
     }
     __syncthreads();
-    const int m = min(PT, g.n - base);
+    const int m = min(NT, g.n - base);
+    // pages given: the last sum that the free ones cover
+    if (t < m && taken <= free_n && (t + 1 == m || s_taken[t + 1] > free_n)) s_given = taken;
     // new pages: page q of the chunk's, asked by request r
-    for (long long q = t; q < sum_taken; q += PT) {
+    for (long long q = t; q < sum_taken; q += NT) {
       const int r = first_above(s_taken, m, carry_taken + q);
       if (s_have[r] < 0) continue;
       const long long at = s_have[r] + carry_taken + q - (r ? s_taken[r - 1] : carry_taken);
@@ -123,7 +145,7 @@ __global__ void __launch_bounds__(PT) plan_kernel(const PlanArgs g) {
     }
     if (g.fill) {
       const int last = (int)min(carry_n + sum_n, (long long)g.total);
-      for (int q = (int)min(carry_n, (long long)g.total) + t; q < last; q += PT) {
+      for (int q = (int)min(carry_n, (long long)g.total) + t; q < last; q += NT) {
         const int r = first_above(s_cu, m, q);
         const int pos = s_len[r] + q - (r ? s_cu[r - 1] : (int)carry_n);
         int slot = -1;
@@ -140,16 +162,15 @@ __global__ void __launch_bounds__(PT) plan_kernel(const PlanArgs g) {
     }
     carry_n += sum_n;
     carry_taken += sum_taken;
-    given += sum_given;
     __syncthreads();                    // the chunk's LDS has been read
   }
   if (g.fill)
-    for (long long q = min(carry_n, (long long)g.total) + t; q < g.total; q += PT) {
+    for (long long q = min(carry_n, (long long)g.total) + t; q < g.total; q += NT) {
       g.slots[q] = -1;
       g.positions[q] = 0;
     }
   __syncthreads();                      // every thread has read the count
-  if (t == 0) *g.free_out = (int)(free_n - given);
+  if (t == 0) *g.free_out = (int)(free_n - s_given);
 }
 
 // The tokens of a large plan, from what plan_kernel left: one thread a token over the whole GPU.
@@ -184,8 +205,10 @@ __global__ void __launch_bounds__(PT) release_kernel(int n, int width, int shift
   for (int base = 0; base < n; base += PT) {
     const int b = base + t;
     const long long len = b < n && release[b] != 0 ? max(lengths[b], 0) : 0;
-    long long pages;
-    s_cum[t] = block_scan(min((len + page - 1) >> shift, (long long)width), part, &pages);
+    long long x[1] = {min((len + page - 1) >> shift, (long long)width)}, sum[1];
+    block_scan<PT>(x, part, sum);
+    s_cum[t] = x[0];
+    const long long pages = sum[0];
     if (b < n && release[b] != 0) lengths[b] = 0;
     __syncthreads();
     const int m = min(PT, n - base);
@@ -198,10 +221,11 @@ __global__ void __launch_bounds__(PT) release_kernel(int n, int width, int shift
         id = *e;
         *e = -1;
       }
-      long long kept;
-      const long long at = top + block_scan(id >= 0 ? 1 : 0, part, &kept) - 1;
+      long long y[1] = {id >= 0 ? 1 : 0}, kept[1];
+      block_scan<PT>(y, part, kept);
+      const long long at = top + y[0] - 1;
       if (id >= 0 && at < capacity) free_pages[at] = id;
-      top = min(top + kept, (long long)capacity);
+      top = min(top + kept[0], (long long)capacity);
     }
     __syncthreads();                    // the chunk's LDS has been read
   }
@@ -373,7 +397,8 @@ hipError_t qtts_paged_plan(int n_requests, int table_width, long long table_stri
              block_table, free_pages, free_capacity, free_count, slots, positions, cu_tokens, kv_lens, lengths_out,
              free_count_out, status, 0};
   g.fill = total_tokens <= 8192;
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(PT), 0, stream, g);
+  if (n_requests <= 256) hipLaunchKernelGGL(plan_kernel<256>, dim3(1), dim3(256), 0, stream, g);
+  else hipLaunchKernelGGL(plan_kernel<PT>, dim3(1), dim3(PT), 0, stream, g);
   if (!g.fill) hipLaunchKernelGGL(plan_tokens_kernel, dim3((unsigned)((total_tokens + 255) / 256)), dim3(256), 0, stream, g);
   return hipGetLastError();
 }
