@@ -435,6 +435,31 @@ hipError_t qtts_paged_attention_prefill(
     long long out_head_stride, const int* block_table, int table_width, long long table_stride,
     const int* kv_lens, const int* cu_tokens, int max_len, float scale, int window, int sinks, hipStream_t stream);
 
+/* The backbone over a paged cache: the new tokens of n_requests streams (any number of streams, any number of
+ * tokens each) through all layers in one call, in the arithmetic of qtts_backbone_prefill but for the
+ * norms and rotation of q and k (f32, one rounding). slots, positions, cu_tokens and kv_lens are a plan's
+ * (qtts_paged_plan); cu_tokens == NULL: one token for each stream, token b of stream b. cache: layer 0's
+ * pages (bf16, 8 heads of 128), layer l's are l * layer_stride elements further. host_layers: the layer
+ * weights' pointers in host memory (layer_weights holds the same on the device). out_hidden: f32
+ * [n_requests, 1024], the final-norm hidden of every stream's last token; zeros for a stream without
+ * tokens or with skip[b] != 0. With codec_head, every stream's token is selected into out_tokens as in
+ * qtts_backbone_step (suppress mask, penalty over history[b * history_stride ..], n_history[b] entries
+ * or history_len where n_history is NULL, EOS, sampling with key seed + b), and out_logits (f32
+ * [n_requests, vocab] or NULL) gets the logits; a skipped stream's stay as they were. Workspace: as
+ * qtts_backbone_prefill's, of qtts_paged_workspace_bytes() bytes. */
+size_t qtts_paged_workspace_bytes(int n_tokens, int n_requests, int vocab, int table_width, int page_size,
+                                  int max_len, int window, int sinks);
+hipError_t qtts_backbone_paged(
+    void* workspace, size_t workspace_bytes, const TTSLayerWeights* layer_weights,
+    const TTSLayerWeights* host_layers, int num_layers, const void* final_norm_weight, const void* cos_table,
+    const void* sin_table, int table_rows, const QttsPagedCache* cache, long long layer_stride, int n_requests,
+    int n_tokens, const int* slots, const int* positions, const int* cu_tokens, const int* kv_lens,
+    const int* block_table, int table_width, long long table_stride, int max_len, int window, int sinks,
+    const void* input_embeddings, float* out_hidden, const void* codec_head, int vocab, float* out_logits,
+    int* out_tokens, int mask_tail, const int* history, int history_stride, const int* n_history,
+    int history_len, float repetition_penalty, int eos_id, int suppress_eos, const QttsSampling* sampling,
+    int frame_step, const int* skip, hipStream_t stream);
+
 /* Debugging aid (no reference counterpart): record the weight-shared kernels' step timeline
  * (s_memrealtime stamps, [256 workgroups][1024 steps][16]: after the entry barrier, after the
  * partials barrier, the end of each of the 8 waves' vector work, 6 points inside a step) into

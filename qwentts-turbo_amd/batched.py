@@ -3,7 +3,7 @@
 Each stream keeps its own backbone KV cache and position; all streams share one copy of the
 weights and one code-predictor decoder. A frame of the batch is two launches per 8 streams: the
 backbone steps (codec head + selection) and the code-predictor frames, queued on the current
-stream with no host sync. Two kernels serve them:
+stream with no host sync. Three ways serve them:
 
 * ``mode="shared"`` (default): the weight-shared kernels. Every weight byte is read once per
   launch for all streams: each workgroup applies its weight tile to the 8 streams' inputs at once
@@ -12,6 +12,9 @@ stream with no host sync. Two kernels serve them:
 * ``mode="per_xcd"``: stream s runs on XCD s alone, its 32 workgroups acting as the 8 virtual
   XCDs of the batch-1 decomposition (every exchange in that XCD's L2), and every stream's results
   are bit-identical to its batch-1 results; each XCD reads the whole weight set for its stream.
+* ``mode="paged"``: any number of streams in one call over one pool of cache pages, in the prompt prefill's bf16
+  arithmetic (``paged.PagedBackbone``); prompts of all streams are prefilled together. Past 8 streams it replaces a
+  launch for every 8.
 
 The reference has no batched decode (its megakernels are batch 1, fused_decode_tts.cu:728-831).
 """
@@ -23,37 +26,56 @@ import torch
 
 from .megakernel_backbone import TTSMegakernelGenerator
 from .megakernel_code_predictor import CodePredictorMegakernelGenerator
+from .paged import PagedBackbone
 
 
 class BatchedTTSDecoder:
     """``n_streams`` backbone decoders over shared weights plus one code predictor."""
 
     MAX_PER_LAUNCH = 8   # streams per launch (one per wave, or one per XCD)
-    MODES = ("shared", "per_xcd")
+    MODES = ("shared", "per_xcd", "paged")
 
     def __init__(self, model, n_streams: int, max_seq_len: int = 4096, cp_max_seq_len: int = 32,
-                 device="cuda", mode: str = "shared"):
+                 device="cuda", mode: str = "shared", *, page_size: int = 64, num_pages: Optional[int] = None,
+                 window: int = 0, sinks: int = 0):
+        """``page_size``, ``num_pages`` (default: enough for every stream at ``max_seq_len``), ``window`` and ``sinks``
+        are ``mode="paged"``'s: its pool of pages, and the sliding window that its tokens attend (0: all)."""
         if n_streams < 1:
             raise ValueError("n_streams must be >= 1")
         if mode not in self.MODES:
             raise ValueError(f"mode={mode!r}: one of {self.MODES}")
+        if mode != "paged" and (window or sinks or num_pages is not None):
+            raise ValueError("num_pages, window and sinks need mode='paged'")
         self.mode = mode
+        self.n_streams = n_streams
+        self.max_seq_len = max_seq_len
+        self.device = torch.device(device)
+        self.paged: Optional[PagedBackbone] = None
+        self.streams: List[TTSMegakernelGenerator] = []
+        if mode == "paged":
+            self.paged = PagedBackbone(model, n_streams, max_seq_len, page_size, num_pages, window, sinks, device)
+            self.vocab_size = self.paged.vocab_size
+            self.cp = CodePredictorMegakernelGenerator(model=model, max_seq_len=cp_max_seq_len, device=device)
+            return
         first = TTSMegakernelGenerator(model=model, max_seq_len=max_seq_len, device=device)
-        self.streams: List[TTSMegakernelGenerator] = [first] + [
+        self.streams = [first] + [
             TTSMegakernelGenerator(max_seq_len=max_seq_len, device=device, shared_weights=first.weights)
             for _ in range(n_streams - 1)]
         self.cp = CodePredictorMegakernelGenerator(model=model, max_seq_len=cp_max_seq_len, device=device)
-        self.n_streams = n_streams
-        self.device = torch.device(device)
         self.vocab_size = self.streams[0].vocab_size
 
     def set_kv_cache(self, stream: int, k: torch.Tensor, v: torch.Tensor):
         """Prefix KV of one stream ([layers, 8, S, 128]); the stream continues at position S."""
+        if self.paged is not None:
+            self.paged.set_kv_cache(stream, k, v)
+            return
         dec = self.streams[stream]
         dec.set_kv_cache(k, v)
         dec.set_position(int(k.shape[2]))
 
     def positions(self) -> List[int]:
+        if self.paged is not None:
+            return list(self.paged.positions)
         return [s.position for s in self.streams]
 
     def step_select(self, embeds: torch.Tensor, tokens_out: torch.Tensor, eos_id: int,
@@ -81,6 +103,19 @@ class BatchedTTSDecoder:
         emb = embeds.to(self.device, torch.bfloat16).contiguous()
         hist = history.to(self.device, torch.int32).contiguous() if history is not None else None
         nh = [int(x) for x in n_history] if n_history else [0] * self.n_streams
+        if self.paged is not None:
+            if len(nh) != self.n_streams or (hist is not None and (hist.dim() != 2 or hist.shape[0] < self.n_streams)):
+                raise ValueError("history must be [n_streams, H] and n_history have one entry per stream")
+            top = hist.shape[1] if hist is not None else 0
+            if any(x < 0 or x > top for x in nh):
+                raise ValueError(f"n_history outside [0, {top}]: {nh}")
+            even = len(set(nh)) == 1
+            return self.paged.forward(
+                emb, [1] * self.n_streams, tokens_out, skip, history=hist,
+                n_history=None if even else torch.tensor(nh, dtype=torch.int32, device=self.device), history_len=nh[0] if even else 0,
+                repetition_penalty=float(repetition_penalty), eos_id=int(eos_id), suppress_eos=bool(suppress_eos),
+                do_sample=bool(do_sample), temperature=float(temperature), top_k=int(top_k), top_p=float(top_p), seed=int(seed),
+                frame_step=int(frame_step))
         # zeros: a skipped stream's row is not written by the kernel
         hidden = torch.zeros(self.n_streams, 1024, dtype=torch.float32, device=self.device)
         lead = self.streams[0].decoder
@@ -115,7 +150,7 @@ class BatchedTTSDecoder:
             self.cp.decoder.frames_streams(hid[b:e], g[b:e], tr[b:e] if tr is not None else None, tokens_out[b:e],
                                            combined_out[b:e], int(eos_id), done[b:e], bool(do_sample),
                                            float(temperature), int(top_k), 1.0, int(seed) + b, int(frame_step),
-                                           self.mode == "shared")
+                                           self.mode != "per_xcd")
 
     def generate(self, talker_input_embeds: Sequence[torch.Tensor], trailing_text_hidden: Sequence[torch.Tensor],
                  tts_pad_embed: torch.Tensor, eos_token_id: int, max_tokens: int = 500, do_sample: bool = False,
@@ -125,17 +160,20 @@ class BatchedTTSDecoder:
                  prefill: str = "mfma") -> List[List[List[int]]]:
         """``NativeTTSGenerator.generate`` (generator.py:77-176) for ``n_streams`` utterances at
         once: one prompt ``[1, seq_s, 1024]`` and one trailing text ``[1, T_s, 1024]`` per stream
-        (ragged lengths), a shared pad row. Each stream is prefilled on its own, then every frame
-        is one code-predictor launch and one backbone launch for all streams, queued with no host
-        sync; the host checks the EOS flags every ``sync_every`` frames and stops when every
+        (ragged lengths), a shared pad row. Each stream is prefilled on its own (``paged``: all together), then every
+        frame is one code-predictor launch and one backbone launch for up to 8 streams (``paged``: one backbone call
+        for all), queued with no host sync; the host checks the EOS flags every ``sync_every`` frames and stops when every
         stream has ended. Stream s samples with key ``seed + s``; in ``per_xcd`` mode it returns
         exactly what a single-stream ``generate(..., seed=seed + s)`` returns for its inputs, in
-        ``shared`` mode the same up to choices that f32 rounding can tip (near-ties)."""
+        ``shared`` mode the same up to choices that f32 rounding can tip (near-ties), in ``paged`` mode up to those
+        that its bf16 arithmetic tips."""
         n = self.n_streams
         if len(talker_input_embeds) != n or len(trailing_text_hidden) != n:
             raise ValueError(f"one prompt and one trailing text per stream ({n}) expected")
         if prefill not in ("mfma", "steps"):
             raise ValueError(f"prefill={prefill!r}: 'mfma' or 'steps'")
+        if prefill == "steps" and self.paged is not None:
+            raise ValueError("mode='paged' prefills all prompts together: prefill='mfma'")
         dev = self.device
         max_tokens = int(max_tokens)
         groups = self.cp.n_groups
@@ -157,16 +195,23 @@ class BatchedTTSDecoder:
             if txt.dim() != 3 or txt.shape[0] != 1 or txt.shape[2] != 1024:
                 raise ValueError(f"trailing text {s} must be [1, T, 1024], got {tuple(txt.shape)}")
             seq = emb.shape[1]
-            if seq < 1 or seq + max_tokens > self.streams[s].max_seq_len:
-                raise ValueError(f"stream {s}: prefill {seq} + max_tokens {max_tokens} exceeds max_seq_len "
-                                 f"{self.streams[s].max_seq_len}")
+            if seq < 1 or seq + max_tokens > self.max_seq_len:
+                raise ValueError(f"stream {s}: prefill {seq} + max_tokens {max_tokens} exceeds max_seq_len {self.max_seq_len}")
+        if self.paged is not None:
+            self.paged.reset()
+            packed = torch.cat([e[0].to(dev, torch.bfloat16) for e in talker_input_embeds])
+            hidden = self.paged.forward(packed, [e.shape[1] for e in talker_input_embeds], g0, eos_id=int(eos_token_id),
+                                        suppress_eos=min_new_tokens > 0, do_sample=bool(do_sample), temperature=float(temperature),
+                                        top_k=int(top_k), top_p=float(top_p), seed=int(seed))
         for s in range(n):
             emb = talker_input_embeds[s]
             seq = emb.shape[1]
-            dec = self.streams[s]
             text = trailing_text_hidden[s][0].to(dev, torch.bfloat16)
             t = min(int(text.shape[0]), max_tokens)
             rows[s, :t] = text[:t]
+            if self.paged is not None:
+                continue
+            dec = self.streams[s]
             e = emb[0].to(dev, torch.bfloat16).contiguous()
             bb = dec.decoder
             bb.reset()
@@ -203,6 +248,11 @@ class BatchedTTSDecoder:
         return out
 
     def check_error(self):
+        if self.paged is not None:
+            self.paged.check_error()
+            self.cp.check_error()
+            self.cp.decoder.check_error_streams()
+            return
         for dec in self.streams:
             dec.check_error()
         self.streams[0].decoder.check_error_streams()

@@ -877,6 +877,102 @@ Tensor paged_attention_prefill(Tensor q, Tensor k_cache, Tensor v_cache, Tensor 
   return o;
 }
 
+// The backbone over a paged cache for any number of streams: weights, and one call per packed batch of new tokens.
+class PagedTTSBackbone {
+ public:
+  PagedTTSBackbone(std::vector<Tensor> layer_weights_flat, Tensor final_norm_weight, Tensor codec_head_weight, Tensor cos_table,
+                   Tensor sin_table, int64_t num_layers)
+      : num_layers_((int)num_layers), dev_(final_norm_weight.device()) {
+    TORCH_CHECK(num_layers >= 1, "num_layers must be >= 1");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev_);
+    TORCH_CHECK(codec_head_weight.dim() == 2, "codec_head_weight must be [vocab, 1024]");
+    check_bf16(codec_head_weight, {codec_head_weight.size(0), kHidden}, "codec_head_weight");
+    check_bf16(final_norm_weight, {kHidden}, "final_norm_weight");
+    TORCH_CHECK(cos_table.dim() == 2 && cos_table.size(0) >= 1 && sin_table.sizes() == cos_table.sizes(), "RoPE tables must be alike");
+    check_bf16(cos_table, {cos_table.size(0), kHeadDim}, "cos_table");
+    check_bf16(sin_table, {sin_table.size(0), kHeadDim}, "sin_table");
+    final_norm_weight_ = final_norm_weight;
+    codec_head_weight_ = codec_head_weight;
+    cos_table_ = cos_table;
+    sin_table_ = sin_table;
+    layers_ = layer_weights_flat;
+    host_ = pack_layers(layer_weights_flat, num_layers_);
+    table_ = upload_struct(host_.data(), host_.size() * sizeof(TTSLayerWeights), dev_);
+  }
+
+  // embeds bf16 [tokens, 1024]; k_pool, v_pool bf16 [layers, pages, 8, page_size, 128]; the plan's tensors (cu_tokens
+  // None: one token for each of kv_lens' streams). Returns the hiddens f32 [streams, 1024]; with out_tokens every stream's
+  // token is selected. history int32 [streams, H] with n_history: an int for all or an int32 tensor [streams].
+  Tensor forward(Tensor embeds, Tensor k_pool, Tensor v_pool, Tensor block_table, Tensor slots, Tensor positions, OptTensor cu_tokens,
+                 Tensor kv_lens, int64_t max_len, int64_t window, int64_t sinks, OptTensor out_tokens, OptTensor history,
+                 OptTensor n_history, int64_t history_len, double repetition_penalty, int64_t eos_id, bool suppress_eos,
+                 bool do_sample, double temperature, int64_t top_k, double top_p, int64_t seed, int64_t frame_step, OptTensor skip,
+                 OptTensor out_logits) {
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(dev_);
+    TORCH_CHECK(k_pool.dim() == 5 && k_pool.size(0) == num_layers_ && v_pool.sizes() == k_pool.sizes() && v_pool.strides() == k_pool.strides(),
+                "k_pool and v_pool must be [", num_layers_, ", pages, 8, page_size, 128], got ", k_pool.sizes());
+    const QttsPagedCache cache = paged_cache(k_pool.select(0, 0), v_pool.select(0, 0));
+    TORCH_CHECK(k_pool.device() == dev_ && cache.dtype == QTTS_BF16 && cache.num_kv_heads == kKVHeads && cache.head_dim == kHeadDim,
+                "the pool must be bfloat16 with 8 heads of 128 on ", dev_);
+    TORCH_CHECK(k_pool.stride(0) % 8 == 0, "pool strides must be multiples of 8");
+    const int64_t n = kv_lens.numel(), tokens = embeds.size(0);
+    TORCH_CHECK(n >= 1 && n <= 65535, "1 .. 65535 streams, got ", n);
+    check_bf16(embeds, {tokens, kHidden}, "embeds");
+    TORCH_CHECK(embeds.device() == dev_ && tokens >= 1 && tokens <= (1 << 20), "embeds must be [1 .. 2^20, 1024] on ", dev_);
+    check_aligned(embeds, "embeds");
+    TORCH_CHECK(cu_tokens.has_value() || tokens == n, "one token for each stream expected (", n, "), got ", tokens);
+    check_table(block_table, dev_, n);
+    TORCH_CHECK(block_table.size(1) <= (INT_MAX - 4096) / cache.page_size, "a block_table row holds more than 2^31 - 4097 tokens");
+    const int width = (int)block_table.size(1);
+    TORCH_CHECK(max_len >= 1 && window >= 0 && window <= INT_MAX && sinks >= 0 && sinks <= INT_MAX, "max_len, window or sinks out of range");
+    const int most = (int)std::min<int64_t>(max_len, (int64_t)width * cache.page_size);
+    int* tok = nullptr;
+    if (out_tokens.has_value()) tok = const_cast<int*>(check_i32(*out_tokens, dev_, n, "out_tokens"));
+    const int* hist = nullptr;
+    int hstride = 0;
+    if (history.has_value()) {
+      hist = check_i32(*history, dev_, 0, "history");
+      TORCH_CHECK(history->dim() == 2 && history->size(0) >= n, "history must be [streams, H]");
+      hstride = (int)history->size(1);
+      TORCH_CHECK(history_len >= 0 && history_len <= hstride, "n_history = ", history_len, " outside [0, ", hstride, "]");
+    }
+    const int vocab = (int)codec_head_weight_.size(0);
+    float* logits = nullptr;
+    if (out_logits.has_value()) {
+      TORCH_CHECK(tok != nullptr, "out_logits needs out_tokens");
+      TORCH_CHECK(out_logits->device() == dev_ && out_logits->scalar_type() == torch::kFloat32 && out_logits->is_contiguous() &&
+                      out_logits->dim() == 2 && out_logits->size(0) == n && out_logits->size(1) == vocab,
+                  "out_logits must be a contiguous f32 [", n, ", ", vocab, "] tensor on ", dev_);
+      logits = out_logits->data_ptr<float>();
+    }
+    const size_t need = qtts_paged_workspace_bytes((int)tokens, (int)n, tok ? vocab : 0, width, cache.page_size, most, (int)window, (int)sinks);
+    TORCH_CHECK(need > 0, "paged workspace size query failed");
+    Tensor ws = torch::empty({(int64_t)need}, torch::dtype(torch::kUInt8).device(dev_));
+    Tensor hidden = torch::empty({n, kHidden}, torch::dtype(torch::kFloat32).device(dev_));
+    QttsSampling samp = sampling(do_sample, temperature, top_k, top_p, seed);
+    hip_check(qtts_backbone_paged(ws.data_ptr(), need, reinterpret_cast<const TTSLayerWeights*>(table_.data_ptr()), host_.data(), num_layers_,
+                                  final_norm_weight_.data_ptr(), cos_table_.data_ptr(), sin_table_.data_ptr(), (int)cos_table_.size(0),
+                                  &cache, k_pool.stride(0), (int)n, (int)tokens, check_i32(slots, dev_, tokens, "slots"),
+                                  check_i32(positions, dev_, tokens, "positions"),
+                                  cu_tokens.has_value() ? check_i32(*cu_tokens, dev_, n + 1, "cu_tokens") : nullptr,
+                                  check_i32(kv_lens, dev_, n, "kv_lens"), block_table.data_ptr<int>(), width, table_stride(block_table), most,
+                                  (int)window, (int)sinks, embeds.data_ptr(), hidden.data_ptr<float>(),
+                                  tok ? codec_head_weight_.data_ptr() : nullptr, vocab, logits, tok, 1, hist, hstride,
+                                  n_history.has_value() ? check_i32(*n_history, dev_, n, "n_history") : nullptr, (int)history_len,
+                                  (float)repetition_penalty, (int)eos_id, suppress_eos ? 1 : 0, &samp, (int)frame_step,
+                                  skip.has_value() ? check_i32(*skip, dev_, n, "skip") : nullptr, cur_stream()),
+              "qtts_backbone_paged");
+    return hidden;
+  }
+
+ private:
+  int num_layers_;
+  torch::Device dev_;
+  std::vector<TTSLayerWeights> host_;
+  std::vector<Tensor> layers_;
+  Tensor final_norm_weight_, codec_head_weight_, cos_table_, sin_table_, table_;
+};
+
 }  // namespace
 
 PYBIND11_MODULE(_qwentts_amd_C, m) {
@@ -908,6 +1004,14 @@ PYBIND11_MODULE(_qwentts_amd_C, m) {
   m.def("paged_attention_prefill", &paged_attention_prefill, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("block_table"), py::arg("kv_lens"), py::arg("cu_tokens"), py::arg("scale"), py::arg("window"), py::arg("sinks"),
         py::arg("max_len"), py::arg("out") = py::none());
+  py::class_<PagedTTSBackbone>(m, "PagedTTSBackbone")
+      .def(py::init<std::vector<Tensor>, Tensor, Tensor, Tensor, Tensor, int64_t>())
+      .def("forward", &PagedTTSBackbone::forward, py::arg("embeds"), py::arg("k_pool"), py::arg("v_pool"), py::arg("block_table"),
+           py::arg("slots"), py::arg("positions"), py::arg("cu_tokens"), py::arg("kv_lens"), py::arg("max_len"), py::arg("window") = 0,
+           py::arg("sinks") = 0, py::arg("out_tokens") = py::none(), py::arg("history") = py::none(), py::arg("n_history") = py::none(),
+           py::arg("history_len") = 0, py::arg("repetition_penalty") = 1.0, py::arg("eos_id") = -1, py::arg("suppress_eos") = false,
+           py::arg("do_sample") = false, py::arg("temperature") = 1.0, py::arg("top_k") = 0, py::arg("top_p") = 1.0,
+           py::arg("seed") = 0, py::arg("frame_step") = 0, py::arg("skip") = py::none(), py::arg("out_logits") = py::none());
   py::class_<MegakernelTTSDecoder>(m, "MegakernelTTSDecoder")
       .def(py::init<torch::Tensor, std::vector<torch::Tensor>, torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor,
                     int64_t, int64_t>())

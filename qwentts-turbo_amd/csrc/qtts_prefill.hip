@@ -667,9 +667,10 @@ __global__ void __launch_bounds__(128 * AKS, 2) attn_pair_kernel(const bf16_t* q
 // rows at one chunk) are conflict-free. Weights are the MFMA's A operand, so a lane ends with 4 consecutive
 // columns of one token: lane l, register e of block (nb, mb) = weight row 16 nb + 4 (l >> 4) + e, token
 // 16 mb + (l & 15). Rows past M read row M - 1; their sums are never stored.
-enum Mode { P_QKV, P_O, P_GU, P_DOWN };
+enum Mode { P_QKV, P_O, P_GU, P_DOWN, P_QKV_PLAIN };   // P_QKV_PLAIN: bf16 q, k, v as projected (paged caches)
+constexpr bool is_qkv(int mode) { return mode == P_QKV || mode == P_QKV_PLAIN; }
 constexpr int kdim(int mode) { return mode == P_O ? NQH * HDIM : (mode == P_DOWN ? INTER : HID); }
-constexpr int ndim(int mode) { return mode == P_QKV ? 4096 : (mode == P_GU ? 2 * INTER : HID); }
+constexpr int ndim(int mode) { return is_qkv(mode) ? 4096 : (mode == P_GU ? 2 * INTER : HID); }
 constexpr int QW = NQH * HDIM;               // a token's rotated queries
 constexpr int SQP = 32;                      // sum-of-squares parts per token (one per column tile)
 
@@ -681,7 +682,7 @@ struct TileArgs {
   int xm, xn;                      // the XCDs as a grid over the tiles: xm x xn = 8
   const float* ssq;                // QKV, GU: [M][SQP] parts of each token's sum(x^2), nsq of them valid
   int nsq;
-  bf16_t* out;                     // QKV: q [M, QW]; GU: [M, INTER]
+  bf16_t* out;                     // QKV: q [M, QW]; plain QKV: q, k, v [M, 4096]; GU: [M, INTER]
   bf16_t* h;                       // O, down: residual stream, updated in place
   bf16_t* xg;                      // ... bf16(h * gain), gain = field nfield of layer nlayer (nlayer < 0: none)
   float* ssq_out;
@@ -701,7 +702,7 @@ template <int MODE, int TN, bool FINE>
 __device__ __forceinline__ const bf16_t* tile_weight_row(const TTSLayerWeights* lw, int tn, int n) {
   constexpr int K = kdim(MODE);
   const int c = tn * TN + n;
-  if constexpr (MODE == P_QKV) {
+  if constexpr (is_qkv(MODE)) {
     return c < 2048 ? tbl(lw, 1) + (size_t)c * K
                     : (c < 3072 ? tbl(lw, 2) + (size_t)(c - 2048) * K : tbl(lw, 3) + (size_t)(c - 3072) * K);
   } else if constexpr (MODE == P_O) {
@@ -806,14 +807,14 @@ __global__ void __launch_bounds__(64 * NWM * NWN * NWK, 2) tile_gemm_kernel(cons
   constexpr int NIW = (TM + TN) / RPI / NW;                 // DMA instructions per wave and stage
   constexpr int STAGE = (TM + TN) * BK * 2;
   constexpr int MB = TM / NWM / 16, NB = TN / NWN / 16;     // a wave's 16 x 16 blocks
-  constexpr bool NORMED = MODE == P_QKV || MODE == P_GU;
+  constexpr bool NORMED = is_qkv(MODE) || MODE == P_GU;
   constexpr int TR = HDIM + 8;                              // QKV: bf16 row of the staged head tile
   static_assert((TM + TN) % (RPI * NW) == 0 && TM % RPI == 0 && K % BK == 0 && NK >= NS - 1, "stages");
   static_assert(KK >= 2 && KK % 2 == 0 && NWK * NWM * NWN == NW, "operand double buffer");
   static_assert(NWK == 1 || (NWK - 1) * TM * TN * 4 <= NS * STAGE, "K parts of the sums");
-  static_assert(MODE != P_QKV || (TN == HDIM && TM * TR * 2 <= NS * STAGE), "QKV: one head per tile");
+  static_assert(!is_qkv(MODE) || (TN == HDIM && TM * TR * 2 <= NS * STAGE), "QKV: one head per tile");
   constexpr bool FINE = MODE == P_GU && (TN / NWN) % 32 != 0;   // gate/up interleave (tile_weight_row)
-  static_assert(ndim(MODE) % TN == 0 && (MODE == P_QKV || MODE == P_GU || ndim(MODE) / TN <= SQP), "column tiles");
+  static_assert(ndim(MODE) % TN == 0 && (NORMED || ndim(MODE) / TN <= SQP), "column tiles");
   // one LDS object: with several, the compiler tracks which of them a DMA may write and waits for every
   // DMA in flight before each LDS read
   __shared__ __attribute__((aligned(1024))) char lds[NS * STAGE + (NORMED ? 1 : NWN) * TM * 4];
@@ -957,10 +958,10 @@ __global__ void __launch_bounds__(64 * NWM * NWN * NWK, 2) tile_gemm_kernel(cons
 #pragma unroll
           for (int mb = 0; mb < MB; ++mb) acc[nb][mb] += *reinterpret_cast<const f32x4*>(part + j * PW + at + (nb * MB + mb) * 256);
     }
-    if constexpr (MODE == P_QKV) __syncthreads();     // the parts have been read: their LDS takes the head tile
+    if constexpr (is_qkv(MODE)) __syncthreads();     // the parts have been read: their LDS takes the head tile
   }
 
-  if constexpr (MODE == P_QKV) {
+  if constexpr (is_qkv(MODE)) {
     bf16_t* T = reinterpret_cast<bf16_t*>(lds);
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
@@ -977,6 +978,14 @@ __global__ void __launch_bounds__(64 * NWM * NWN * NWK, 2) tile_gemm_kernel(cons
     }
     __syncthreads();
     const int head = tn;   // q heads 0..15, k heads 16..23, v heads 24..31
+    if constexpr (MODE == P_QKV_PLAIN) {
+      for (int q = t; q < TM * 16; q += NT) {
+        const int row = q >> 4, ch = 8 * (q & 15), m = m0 + row;
+        if (m < g.M)
+          *reinterpret_cast<u32x4*>(g.out + (size_t)m * ndim(MODE) + head * HDIM + ch) = *reinterpret_cast<const u32x4*>(T + row * TR + ch);
+      }
+      return;
+    }
     if (head >= NQH + NKVH) {
       bf16_t* vbase = g.vc + ((size_t)g.layer * NKVH + (head - NQH - NKVH)) * g.max_seq * HDIM;
       for (int q = t; q < TM * 16; q += NT) {
@@ -1116,6 +1125,112 @@ __global__ void __launch_bounds__(64) select_kernel(const bf16_t* logits, int n,
   if (lane == 0) *out_token = tok;
 }
 
+// The final norm of every request's last token (row cu[b + 1] - 1; NULL: row b), one wave a request: hidden, and the
+// same as bf16 for the head. A request without tokens or skipped gets a row of zeros.
+__global__ void __launch_bounds__(64) last_norm_kernel(const bf16_t* h, const bf16_t* gain, const int* cu, int M, const int* skip,
+                                                       float* out_hidden, bf16_t* y) {
+  const int lane = threadIdx.x, b = blockIdx.x;
+  const int row = cu != nullptr ? cu[b + 1] - 1 : b;
+  const bool none = row < 0 || row >= M || (cu != nullptr && row < cu[b]) || (skip != nullptr && skip[b] != 0);
+  const bf16_t* x = h + (size_t)(none ? 0 : row) * HID;
+  u32x4 v[2], gw[2];
+  float ss = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    v[k] = ldw(x + 8 * (lane + 64 * k));
+    gw[k] = ldw(gain + 8 * (lane + 64 * k));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ss += bflo(v[k][e]) * bflo(v[k][e]) + bfhi(v[k][e]) * bfhi(v[k][e]);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) ss += __shfl_xor(ss, o, 64);
+  const float rs = 1.0f / sqrtf(ss / (float)HID + EPS);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int e0 = 8 * (lane + 64 * k);
+    u32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float a = none ? 0.0f : rbh(bflo(gw[k][e]) * rbh(bflo(v[k][e]) * rs));
+      const float c = none ? 0.0f : rbh(bfhi(gw[k][e]) * rbh(bfhi(v[k][e]) * rs));
+      out_hidden[(size_t)b * HID + e0 + 2 * e] = a;
+      out_hidden[(size_t)b * HID + e0 + 2 * e + 1] = c;
+      o[e] = pack_bh(a, c);
+    }
+    *reinterpret_cast<u32x4*>(y + (size_t)b * HID + e0) = o;
+  }
+}
+
+// Codec-head logits of all requests: a wave keeps RPW rows of the head and takes HRB requests.
+constexpr int HRB = 16;
+__global__ void __launch_bounds__(256) rows_head_kernel(const bf16_t* y, int n, const bf16_t* head, int vocab, bf16_t* logits) {
+  const int lane = threadIdx.x & 63, w = blockIdx.x * 4 + (threadIdx.x >> 6);
+  u32x4 hw[RPW][2];
+#pragma unroll
+  for (int r = 0; r < RPW; ++r)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) hw[r][k] = ldw(head + (size_t)min(RPW * w + r, vocab - 1) * HID + 8 * (lane + 64 * k));
+  for (int b = HRB * blockIdx.y; b < min(n, HRB * ((int)blockIdx.y + 1)); ++b) {
+    float s[RPW];
+    u32x4 x[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) x[k] = ldw(y + (size_t)b * HID + 8 * (lane + 64 * k));
+#pragma unroll
+    for (int r = 0; r < RPW; ++r) {
+      s[r] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[r] += bflo(hw[r][k][e]) * bflo(x[k][e]) + bfhi(hw[r][k][e]) * bfhi(x[k][e]);
+    }
+    group_sum_n<64>(s);
+#pragma unroll
+    for (int r = 0; r < RPW; ++r)
+      if (lane == r && RPW * w + r < vocab) logits[(size_t)b * vocab + RPW * w + r] = f2bh(s[r]);
+  }
+}
+
+// select_kernel for every request, with the repetition penalty over its history (bf16 arithmetic, once per id,
+// generator.py:161-167): stream b draws with key sp.seed + b; a skipped request's token and logits stay as they were.
+__global__ void __launch_bounds__(64) rows_select_kernel(const bf16_t* logits, int n, int mask_tail, int eos_id, int suppress_eos,
+                                                         const int* history, int history_stride, const int* n_history,
+                                                         int history_len, float penalty, SelParams sp, const int* skip,
+                                                         float* out_logits, int* out_token) {
+  __shared__ SelScratch sc;
+  __shared__ uint32_t seen[SEL_NJ * 2];
+  const int lane = threadIdx.x, b = blockIdx.x;
+  if (skip != nullptr && skip[b] != 0) return;
+  const bool pen = penalty != 1.0f && history != nullptr;
+  if (pen) {
+    for (int i = lane; i < SEL_NJ * 2; i += 64) seen[i] = 0u;
+    __syncthreads();
+    const int len = min(max(n_history != nullptr ? n_history[b] : history_len, 0), history_stride);
+    for (int i = lane; i < len; i += 64) {
+      const int id = history[(size_t)b * history_stride + i];
+      if (id >= 0 && id < n) atomicOr(&seen[id >> 5], 1u << (id & 31));
+    }
+    __syncthreads();
+  }
+  logits += (size_t)b * n;
+  bf16_t lv[SEL_NJ];
+#pragma unroll
+  for (int j = 0; j < SEL_NJ; ++j) lv[j] = *gmem(logits + min(lane + 64 * j, n - 1));
+  uint32_t w[SEL_NJ], best = 0u;
+#pragma unroll
+  for (int j = 0; j < SEL_NJ; ++j) {
+    const int i = lane + 64 * j;
+    float v = bf2f(lv[j]);
+    if (out_logits && i < n) out_logits[(size_t)b * n + i] = v;
+    if (pen && i < n && ((seen[i >> 5] >> (i & 31)) & 1u)) v = rbh(v > 0.0f ? v / penalty : v * penalty);
+    if ((mask_tail && i >= n - 1024 && i != eos_id) || (suppress_eos && i == eos_id)) v = -INFINITY;
+    w[j] = i < n ? (bfkey(v) << 16) | (uint32_t)i : 0u;
+    best = max(best, i < n ? greedy_word(v, i) : 0u);
+  }
+  sp.seed += (unsigned long long)b;
+  const int tok = sp.do_sample ? wave_sample(w, n, sp, &sc) : greedy_id(best, n);
+  if (lane == 0) out_token[b] = tok;
+}
+
 // ---- host ----------------------------------------------------------------------------------
 
 // One launch of a projection: tile TM x TN (NWM x NWN waves), NS stages of BK.
@@ -1156,12 +1271,13 @@ void launch_tile(TileArgs& g, hipStream_t st) {
 //   GU    128 x 128 to 2688 (two rounds of 512): 2049 46.4 : 41.3, 2560 55.0 : 46.3 (3072 56.5 : 58.9)
 //   O, D  128 x 64, no K shares: O 2049 33.2 : 24.6, 3072 36.8 : 32.0, 6000 74.6 : 65.3; down 43.6 : 35.4,
 //         49.6 : 43.8, 100.4 : 92.1
+template <int MODE>
 void project_qkv(TileArgs& g, hipStream_t st) {
-  if (g.M <= 256) launch_tile<P_QKV, 32, 128, 1, 4, 1, 6, 64>(g, st);
-  else if (g.M <= 512) launch_tile<P_QKV, 64, 128, 2, 2, 1, 5, 64>(g, st);
-  else if (g.M <= 1024) launch_tile<P_QKV, 128, 128, 4, 2, 1, 4, 64>(g, st);
-  else if (g.M > 2048 && g.M <= 4096) launch_tile<P_QKV, 128, 128, 2, 2, 1, 2, 64>(g, st);
-  else launch_tile<P_QKV, 256, 128, 4, 2, 1, 3, 64>(g, st);
+  if (g.M <= 256) launch_tile<MODE, 32, 128, 1, 4, 1, 6, 64>(g, st);
+  else if (g.M <= 512) launch_tile<MODE, 64, 128, 2, 2, 1, 5, 64>(g, st);
+  else if (g.M <= 1024) launch_tile<MODE, 128, 128, 4, 2, 1, 4, 64>(g, st);
+  else if (g.M > 2048 && g.M <= 4096) launch_tile<MODE, 128, 128, 2, 2, 1, 2, 64>(g, st);
+  else launch_tile<MODE, 256, 128, 4, 2, 1, 3, 64>(g, st);
 }
 void project_gate_up(TileArgs& g, hipStream_t st) {
   if (g.M <= 32) launch_tile<P_GU, 16, 64, 1, 4, 1, 4, 128>(g, st);
@@ -1202,6 +1318,26 @@ Layout layout(int S, int vocab) {
   L.att = take((size_t)S * QW * 2);
   L.act = take((size_t)S * INTER * 2);
   L.logits = take((size_t)(vocab > 0 ? vocab : MAXV) * 2);
+  L.total = o;
+  return L;
+}
+
+// Workspace of qtts_backbone_paged: the prefill's activations, then q, k, v as projected, the decode attention's
+// partial sums, the requests' normed rows and their logits.
+struct PagedLayout {
+  Layout p;
+  size_t qkv, part, part_bytes, y, logits, total;
+};
+PagedLayout paged_layout(int n_tokens, int n_requests, int vocab, size_t part_bytes) {
+  PagedLayout L;
+  L.p = layout(n_tokens, 0);
+  size_t o = L.p.total;
+  auto take = [&](size_t bytes) { const size_t at = o; o = align256(o + bytes); return at; };
+  L.qkv = take((size_t)n_tokens * ndim(P_QKV_PLAIN) * 2);
+  L.part = take(part_bytes);
+  L.part_bytes = part_bytes;
+  L.y = take((size_t)n_requests * HID * 2);
+  L.logits = take((size_t)n_requests * vocab * 2);
   L.total = o;
   return L;
 }
@@ -1271,7 +1407,7 @@ hipError_t qtts_backbone_prefill(void* workspace, size_t workspace_bytes, const 
   for (int l = 0; l < num_layers; ++l) {
     g.layer = l;
     g.A = xg; g.out = q;
-    project_qkv(g, stream);
+    project_qkv<P_QKV>(g, stream);
     // the two-head kernel for prompts that fill the chip with half the workgroups; below, the per-head kernel
     // and its reads ahead (us a layer, per head against two heads: 640 tokens 69.2 : 75.2, 768 72.0 : 76.9,
     // 1000 79.4 : 81.6, 1280 111.1 : 116.2, 1500 117.0 : 118.4, 2048 141.5 : 137.4, 3000 248.2 : 246.4; with a
@@ -1307,6 +1443,109 @@ hipError_t qtts_backbone_prefill(void* workspace, size_t workspace_bytes, const 
     sp.group = 0;
     hipLaunchKernelGGL(select_kernel, dim3(1), dim3(64), 0, stream, lg, vocab, mask_tail, eos_id, suppress_eos, sp,
                        out_logits, out_token);
+  }
+  return hipGetLastError();
+}
+
+size_t qtts_paged_workspace_bytes(int n_tokens, int n_requests, int vocab, int table_width, int page_size, int max_len, int window,
+                                  int sinks) {
+  if (n_tokens < 1 || n_requests < 1 || vocab < 0 || vocab > MAXV || table_width < 1 || page_size < 1 || max_len < 1 ||
+      window < 0 || sinks < 0)
+    return 0;
+  return paged_layout(n_tokens, n_requests, vocab,
+                      qtts_paged_decode_workspace_bytes(n_requests, NQH, NKVH, HDIM, table_width, page_size, max_len, window, sinks))
+      .total;
+}
+
+hipError_t qtts_backbone_paged(void* workspace, size_t workspace_bytes, const TTSLayerWeights* layer_weights,
+                               const TTSLayerWeights* host_layers, int num_layers, const void* final_norm_weight, const void* cos_table, const void* sin_table, int table_rows,
+                               const QttsPagedCache* cache, long long layer_stride, int n_requests, int n_tokens,
+                               const int* slots, const int* positions, const int* cu_tokens, const int* kv_lens,
+                               const int* block_table, int table_width, long long table_stride, int max_len, int window,
+                               int sinks, const void* input_embeddings, float* out_hidden, const void* codec_head, int vocab,
+                               float* out_logits, int* out_tokens, int mask_tail, const int* history, int history_stride,
+                               const int* n_history, int history_len, float repetition_penalty, int eos_id, int suppress_eos,
+                               const QttsSampling* sampling, int frame_step, const int* skip, hipStream_t stream) {
+  if (workspace == nullptr || layer_weights == nullptr || host_layers == nullptr || final_norm_weight == nullptr ||
+      cos_table == nullptr || sin_table == nullptr || cache == nullptr || slots == nullptr || positions == nullptr || kv_lens == nullptr ||
+      block_table == nullptr || input_embeddings == nullptr || out_hidden == nullptr)
+    return hipErrorInvalidValue;
+  if (num_layers < 1 || n_requests < 1 || n_tokens < 1 || n_tokens > (1 << 20) || n_requests > 65535 * HRB || table_rows < 1 || max_len < 1 || window < 0 ||
+      sinks < 0 || layer_stride < 0 || (layer_stride & 7) != 0)
+    return hipErrorInvalidValue;
+  if (cache->dtype != QTTS_BF16 || cache->num_kv_heads != NKVH || cache->head_dim != HDIM || table_width < 1 || cache->page_size < 16)
+    return hipErrorInvalidValue;
+  if (cu_tokens == nullptr && n_tokens != n_requests) return hipErrorInvalidValue;   // (one token each, in order)
+  if (codec_head != nullptr && (vocab < 128 || vocab > MAXV || vocab % 128 != 0 || out_tokens == nullptr)) return hipErrorInvalidValue;
+  if (history != nullptr && history_stride < 0) return hipErrorInvalidValue;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0 || (reinterpret_cast<uintptr_t>(input_embeddings) & 15u) != 0)
+    return hipErrorInvalidValue;
+  const bool single = cu_tokens == nullptr;
+  const size_t part = qtts_paged_decode_workspace_bytes(n_requests, NQH, NKVH, HDIM, table_width, cache->page_size, max_len, window, sinks);
+  const PagedLayout L = paged_layout(n_tokens, n_requests, codec_head ? vocab : 0, part);
+  if (workspace_bytes < L.total) return hipErrorInvalidValue;
+  char* ws = static_cast<char*>(workspace);
+  bf16_t* h = reinterpret_cast<bf16_t*>(ws + L.p.h);
+  bf16_t* xg = reinterpret_cast<bf16_t*>(ws + L.p.xg);
+  float* ssq = reinterpret_cast<float*>(ws + L.p.ssq);
+  bf16_t* q = reinterpret_cast<bf16_t*>(ws + L.p.q);
+  bf16_t* att = reinterpret_cast<bf16_t*>(ws + L.p.att);
+  bf16_t* act = reinterpret_cast<bf16_t*>(ws + L.p.act);
+  bf16_t* qkv = reinterpret_cast<bf16_t*>(ws + L.qkv);
+  bf16_t* y = reinterpret_cast<bf16_t*>(ws + L.y);
+  const float scale = 1.0f / sqrtf((float)HDIM);
+  constexpr int QKV = ndim(P_QKV_PLAIN), KOFF = NQH * HDIM, VOFF = KOFF + NKVH * HDIM;
+  hipLaunchKernelGGL(embed_kernel, dim3((unsigned)((n_tokens + 3) / 4)), dim3(256), 0, stream,
+                     static_cast<const bf16_t*>(input_embeddings), layer_weights, h, xg, ssq, n_tokens);
+  TileArgs g{};
+  g.layers = layer_weights;
+  g.M = n_tokens;
+  g.ssq = ssq;
+  g.ssq_out = ssq;
+  g.h = h;
+  g.xg = xg;
+  g.nsq = 1;   // the embeddings' sums of squares are whole
+  QttsPagedCache kv = *cache;
+  for (int l = 0; l < num_layers; ++l) {
+    g.layer = l;
+    g.A = xg; g.out = qkv;
+    project_qkv<P_QKV_PLAIN>(g, stream);
+    kv.k = static_cast<bf16_t*>(cache->k) + (long long)l * layer_stride;
+    kv.v = static_cast<bf16_t*>(cache->v) + (long long)l * layer_stride;
+    hipError_t e = qtts_qk_norm_rope_store(&kv, n_tokens, NQH, qkv, QKV, HDIM, qkv + KOFF, QKV, HDIM, qkv + VOFF, QKV, HDIM, q, QW,
+                                           HDIM, host_layers[l].q_norm_weight, host_layers[l].k_norm_weight, EPS, cos_table,
+                                           sin_table, 0, table_rows, positions, 0, 0, 0, slots, stream);
+    if (e != hipSuccess) return e;
+    if (single)
+      e = qtts_paged_attention_decode(&kv, n_requests, NQH, q, QW, HDIM, att, QW, HDIM, block_table, table_width, table_stride,
+                                      kv_lens, max_len, scale, window, sinks, part > 0 ? ws + L.part : nullptr, part, stream);
+    else
+      e = qtts_paged_attention_prefill(&kv, n_requests, n_tokens, NQH, q, QW, HDIM, att, QW, HDIM, block_table, table_width,
+                                       table_stride, kv_lens, cu_tokens, max_len, scale, window, sinks, stream);
+    if (e != hipSuccess) return e;
+    g.A = att; g.nlayer = l; g.nfield = 7;
+    project_residual<P_O>(g, stream);
+    g.A = xg; g.out = act;
+    project_gate_up(g, stream);
+    g.A = act; g.nlayer = l + 1 < num_layers ? l + 1 : -1; g.nfield = 0;
+    project_residual<P_DOWN>(g, stream);
+  }
+  hipLaunchKernelGGL(last_norm_kernel, dim3((unsigned)n_requests), dim3(64), 0, stream, h, static_cast<const bf16_t*>(final_norm_weight),
+                     cu_tokens, n_tokens, skip, out_hidden, y);
+  if (codec_head != nullptr) {
+    bf16_t* lg = reinterpret_cast<bf16_t*>(ws + L.logits);
+    hipLaunchKernelGGL(rows_head_kernel, dim3((vocab + 4 * RPW - 1) / (4 * RPW), (n_requests + HRB - 1) / HRB), dim3(256), 0, stream,
+                       y, n_requests, static_cast<const bf16_t*>(codec_head), vocab, lg);
+    SelParams sp{};
+    sp.do_sample = sampling ? sampling->do_sample : 0;
+    sp.temperature = sampling ? sampling->temperature : 1.0f;
+    sp.top_k = sampling ? sampling->top_k : 0;
+    sp.top_p = sampling ? sampling->top_p : 1.0f;
+    sp.seed = sampling ? sampling->seed : 0ull;
+    sp.frame_step = frame_step;
+    sp.group = 0;
+    hipLaunchKernelGGL(rows_select_kernel, dim3((unsigned)n_requests), dim3(64), 0, stream, lg, vocab, mask_tail, eos_id, suppress_eos,
+                       history, history_stride, n_history, history_len, repetition_penalty, sp, skip, out_logits, out_tokens);
   }
   return hipGetLastError();
 }

@@ -5,18 +5,20 @@ A layer's cache is two tensors ``[pages, kv_heads, page_size, head_dim]`` (bf16 
 ``page * page_size + place in the page``. The reference has one contiguous cache for one stream
 (megakernel_backbone.py:156-159). ``csrc/qtts_paged.hip`` and ``csrc/qtts_paged_attn.hip`` hold the kernels.
 
-A step of a batch is ``paged_plan`` once, then per layer ``qk_norm_rope_store`` and
+``BatchedTTSDecoder(mode="paged")`` serves any number of streams this way (``PagedBackbone`` below). By hand, a
+step of a batch is ``paged_plan`` once, then per layer ``qk_norm_rope_store`` and
 ``paged_attention_decode`` (one new token per request) or ``paged_attention_prefill`` (any number).
 Every call queues on the current stream, reads lengths and tables on the device, keeps no state and may be
 captured into a graph (the shapes are then fixed, the lengths are not).
 """
 from __future__ import annotations
 
-from typing import NamedTuple, Optional, Sequence
+from typing import List, NamedTuple, Optional, Sequence
 
 import torch
 
 from . import _ext
+from .weights import HEAD_DIM, HIDDEN_SIZE, NUM_KV_HEADS
 
 
 class PagedPlan(NamedTuple):
@@ -93,3 +95,107 @@ def _scale(scale, q):
 
 def _max_len(max_len, block_table, k_cache):
     return int(max_len) if max_len is not None else max(1, block_table.shape[-1] * k_cache.shape[-2])
+
+
+class PagedBackbone:
+    """The backbone's streams over one pool of pages: ``BatchedTTSDecoder``'s ``mode="paged"``.
+
+    All streams' new tokens go through the layers in one call (``qtts_backbone_paged``: the MFMA projections of the
+    prompt prefill around the operators above), whether they are prompts or single tokens. Pages are taken as
+    streams grow, so a pool may be smaller than ``n_streams * max_seq_len``; when it runs out, the streams that
+    found no page are noted on the device and ``check_error`` raises. ``window`` > 0 bounds what a token attends
+    (its last ``window`` keys and the first ``sinks``); pages behind the window stay with their stream."""
+
+    def __init__(self, model, n_streams: int, max_seq_len: int = 4096, page_size: int = 64, num_pages: Optional[int] = None,
+                 window: int = 0, sinks: int = 0, device="cuda"):
+        from .megakernel_backbone import _extract_tts_backbone_weights
+        if page_size < 16 or page_size > 65536 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two in [16, 65536], got {page_size}")
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks must be >= 0")
+        self.width = -(-max_seq_len // page_size)
+        self.num_pages = n_streams * self.width if num_pages is None else int(num_pages)
+        if self.num_pages < 1:
+            raise ValueError("num_pages must be >= 1")
+        w = _extract_tts_backbone_weights(model, max_seq_len, device=device)
+        self.kernel = _ext.load().PagedTTSBackbone(w["layer_weights"], w["final_norm_weight"], w["codec_head_weight"], w["cos_table"],
+                                                   w["sin_table"], w["num_layers"])
+        self.vocab_size, self.num_layers = w["vocab_size"], w["num_layers"]
+        self.n_streams, self.max_seq_len, self.page_size = n_streams, max_seq_len, page_size
+        self.window, self.sinks = int(window), int(sinks)
+        self.device = torch.device(device)
+        pool = (self.num_layers, self.num_pages, NUM_KV_HEADS, page_size, HEAD_DIM)
+        self.k_pool = torch.empty(pool, dtype=torch.bfloat16, device=device)
+        self.v_pool = torch.empty(pool, dtype=torch.bfloat16, device=device)
+        i32 = dict(dtype=torch.int32, device=device)
+        self.block_table = torch.full((n_streams, self.width), -1, **i32)
+        self.lengths = torch.zeros(n_streams, **i32)
+        self.free_pages = torch.arange(self.num_pages, **i32)
+        self.free_count = torch.full((1,), self.num_pages, **i32)
+        self.failed = torch.zeros(n_streams, **i32)        # largest plan status of each stream
+        self._ones = torch.ones(n_streams, **i32)
+        self.positions: List[int] = [0] * n_streams        # tokens asked for, by the host's count
+
+    def reset(self, streams: Optional[Sequence[int]] = None) -> None:
+        """Gives the pages of ``streams`` (default: all) back; they start again at position 0."""
+        which = range(self.n_streams) if streams is None else streams
+        flags = [0] * self.n_streams
+        for s in which:
+            flags[s] = 1
+            self.positions[s] = 0
+        mask = torch.tensor(flags, dtype=torch.int32, device=self.device)
+        paged_release(mask, self.lengths, self.block_table, self.free_pages, self.free_count, self.page_size)
+        self.failed.masked_fill_(mask != 0, 0)
+
+    def _plan(self, counts: Sequence[int]) -> PagedPlan:
+        for s, n in enumerate(counts):
+            if self.positions[s] + n > self.max_seq_len:
+                raise RuntimeError(f"stream {s}: position {self.positions[s]} + {n} tokens exceeds max_seq_len {self.max_seq_len} "
+                                   "(KV cache full)")
+        new = self._ones if all(n == 1 for n in counts) else torch.tensor(list(counts), dtype=torch.int32, device=self.device)
+        plan = paged_plan(new, self.lengths, self.block_table, self.free_pages, self.free_count, self.page_size, sum(counts))
+        torch.maximum(self.failed, plan.status, out=self.failed)
+        for s, n in enumerate(counts):
+            self.positions[s] += n
+        return plan
+
+    def set_kv_cache(self, stream: int, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Prefix K and V ([layers, 8, S, 128]) of one stream, which continues at position S."""
+        shape = (self.num_layers, NUM_KV_HEADS, k.shape[2] if k.dim() == 4 else -1, HEAD_DIM)
+        if tuple(k.shape) != shape or v.shape != k.shape:
+            raise ValueError(f"k and v must be [{self.num_layers}, {NUM_KV_HEADS}, S, {HEAD_DIM}], got {tuple(k.shape)} and {tuple(v.shape)}")
+        self.reset([stream])
+        counts = [0] * self.n_streams
+        counts[stream] = int(k.shape[2])
+        slots = self._plan(counts).slots.long()
+        if not bool((slots >= 0).all()):
+            raise RuntimeError(f"stream {stream}: the pool has too few free pages for {counts[stream]} tokens")
+        page, place = slots // self.page_size, slots % self.page_size
+        for pool, x in ((self.k_pool, k), (self.v_pool, v)):
+            pool[:, page, :, place] = x.to(self.device, torch.bfloat16).permute(2, 0, 1, 3)
+
+    def forward(self, embeds: torch.Tensor, counts: Sequence[int], out_tokens: Optional[torch.Tensor] = None,
+                skip: Optional[torch.Tensor] = None, **select) -> torch.Tensor:
+        """``counts[s]`` new tokens of every stream s, their embeddings packed in ``embeds`` (bf16 [sum, 1024]), through
+        all layers. Returns the final-norm hidden of each stream's last token (f32 [n_streams, 1024]; zeros for a
+        stream without tokens or skipped). With ``out_tokens`` each stream's token is selected (``select``: the
+        arguments of ``step_select``). ``skip`` needs one token for every stream."""
+        single = all(n == 1 for n in counts)
+        if skip is not None and not single:
+            raise ValueError("skip needs one token for every stream")
+        if embeds.shape != (sum(counts), HIDDEN_SIZE):
+            raise ValueError(f"embeds must be [{sum(counts)}, {HIDDEN_SIZE}], got {tuple(embeds.shape)}")
+        plan = self._plan(counts)
+        slots, lens = plan.slots, plan.kv_lens
+        if skip is not None:            # a finished stream stores and attends nothing
+            slots = torch.where(skip != 0, -1, slots)
+            lens = torch.where(skip != 0, 0, lens)
+        return self.kernel.forward(embeds, self.k_pool, self.v_pool, self.block_table, slots, plan.positions,
+                                   None if single else plan.cu_tokens, lens, max(self.positions), self.window, self.sinks,
+                                   out_tokens=out_tokens, skip=skip, **select)
+
+    def check_error(self) -> None:
+        """Raises if the pool had no page for some stream since its last reset (synchronises)."""
+        bad = [s for s, x in enumerate(self.failed.tolist()) if x]
+        if bad:
+            raise RuntimeError(f"paged cache: no free page for streams {bad} (pool of {self.num_pages} pages); reset them")
