@@ -384,3 +384,163 @@ def test_results_repeat_bit_for_bit(pkg):
     first = pkg.paged_attention_decode(q, k, v, ints(table), ints(lens))
     for _ in range(5):
         assert torch.equal(first, pkg.paged_attention_decode(q, k, v, ints(table), ints(lens)))
+
+
+# ---- refusals, streams, graphs -------------------------------------------------------------------
+
+
+def test_refusals(pkg):
+    """Every call that a kernel could not carry out raises, and nothing is written."""
+    k = torch.zeros(4, 8, 16, 128, dtype=torch.bfloat16, device=DEV)
+    v = torch.zeros_like(k)
+    q = torch.zeros(3, 16, 128, dtype=torch.bfloat16, device=DEV)
+    t, lens, cu = ints([[0, 1], [2, 3], [0, 0]]), ints([1, 2, 3]), ints([0, 1, 2, 3])
+    tab = torch.zeros(9, 128, dtype=torch.bfloat16, device=DEV)
+    pos = ints([0, 1, 2])
+
+    def decode(**kw):
+        a = dict(q=q, k_cache=k, v_cache=v, block_table=t, kv_lens=lens)
+        a.update(kw)
+        return pkg.paged_attention_decode(**a)
+
+    def prefill(**kw):
+        a = dict(q=q, k_cache=k, v_cache=v, block_table=t, kv_lens=lens, cu_tokens=cu)
+        a.update(kw)
+        return pkg.paged_attention_prefill(**a)
+
+    def store(**kw):
+        a = dict(q=q, k=q[:, :8], v=q[:, :8], q_weight=None, k_weight=None, cos=tab, sin=tab, positions=pos, slots=pos, k_cache=k, v_cache=v)
+        a.update(kw)
+        return pkg.qk_norm_rope_store(**a)
+
+    both = [dict(q=q.half()), dict(q=q[:, :12]), dict(q=q[..., :64]), dict(q=q.cpu()), dict(v_cache=v[:2]), dict(v_cache=v.half()),
+            dict(k_cache=k.float(), v_cache=v.float()), dict(k_cache=k[:, :, :12], v_cache=v[:, :, :12]),
+            dict(k_cache=k[..., :96], v_cache=v[..., :96]), dict(block_table=t.long()), dict(block_table=t[0]), dict(block_table=t.T),
+            dict(block_table=t.cpu()), dict(kv_lens=lens.long()), dict(kv_lens=lens[:2]), dict(scale=0.0), dict(scale=-1.0),
+            dict(scale=float("nan")), dict(window=-1), dict(sinks=-2), dict(max_len=0), dict(out=q[:2]), dict(out=q.half()),
+            dict(q=torch.zeros(3, 16, 256, dtype=torch.bfloat16, device=DEV)[..., ::2]),
+            dict(q=torch.zeros(3 * 16 * 128 + 1, dtype=torch.bfloat16, device=DEV)[1:].view(3, 16, 128))]
+    for bad in both:
+        with pytest.raises(RuntimeError):
+            decode(**bad)
+        with pytest.raises(RuntimeError):
+            prefill(**bad)
+    with pytest.raises(RuntimeError):
+        prefill(cu_tokens=cu.long())
+    with pytest.raises(RuntimeError):
+        prefill(cu_tokens=ints([0, 1, 2, 3, 3]))          # four requests, three lengths
+    for bad in (dict(k=q), dict(v=q[:2, :8]), dict(q=q.half()), dict(cos=tab[:, :64]), dict(sin=tab[:4]), dict(cos=tab.half()), dict(positions=pos[:2]),
+                dict(positions=pos.long()), dict(positions=torch.stack([pos, pos])), dict(slots=pos[:2]), dict(slots=ints([0, 1, 2, 3])),
+                dict(slots=pos.cpu()), dict(q_weight=tab[0, :64]), dict(k_weight=tab[0].float()), dict(eps=-1.0), dict(out=q[:, :8]),
+                dict(positions=torch.stack([pos] * 3), mrope_section=(24, 20, 21)),
+                dict(positions=torch.stack([pos] * 3), mrope_section=(0, 32, 32))):
+        with pytest.raises(RuntimeError):
+            store(**bad)
+    one = ints([1])
+    for bad in (dict(new_tokens=one.long()), dict(lengths=ints([])), dict(block_table=ints([1])), dict(page_size=24), dict(page_size=0),
+                dict(total_tokens=-1), dict(free_count=ints([])), dict(lengths_out=one.cpu())):
+        a = dict(new_tokens=one, lengths=ints([0]), block_table=ints([[-1]]), free_pages=ints([3]), free_count=ints([1]), page_size=16, total_tokens=1)
+        a.update(bad)
+        with pytest.raises(RuntimeError):
+            pkg.paged_plan(**a)
+    assert bool((k == 0).all()) and bool((v == 0).all())
+    assert store().shape == (3, 16, 128) and decode().shape == (3, 16, 128)
+
+
+def step_state(seed, dtype=torch.bfloat16):
+    """A batch before a step: pages, lengths and one layer's cache."""
+    g = gen(seed)
+    lens = [37, 0, 300, 64]
+    k, v, table = make_cache(g, lens, 16, 8, 128, dtype, spare=40, width=24)
+    used = {p for row in table for p in row}
+    free = [p for p in range(k.shape[0]) if p not in used]
+    angle = torch.rand(400, 64, generator=g, device=DEV) * 6
+    cos, sin = (torch.cat((f(angle), f(angle)), -1).to(dtype) for f in (torch.cos, torch.sin))
+    qkv = torch.randn(4, 32, 128, generator=g, device=DEV).to(dtype)
+    w = torch.ones(128, dtype=dtype, device=DEV)
+    return dict(k=k, v=v, table=ints(table), lens=ints(lens), free=ints(free), count=ints([len(free)]), cos=cos, sin=sin, qkv=qkv, w=w,
+                new=ints([1, 1, 1, 1]))
+
+
+def step(pkg, s, max_len=None):
+    """One layer's step as a server runs it: plan, store, attend (lengths grow in place)."""
+    p = pkg.paged_plan(s["new"], s["lens"], s["table"], s["free"], s["count"], 16, 4)
+    q, k, v = s["qkv"][:, :16], s["qkv"][:, 16:24], s["qkv"][:, 24:]
+    q = pkg.qk_norm_rope_store(q, k, v, s["w"], s["w"], s["cos"], s["sin"], p.positions, p.slots, s["k"], s["v"])
+    a = pkg.paged_attention_decode(q, s["k"], s["v"], s["table"], p.kv_lens, max_len=max_len)
+    b = pkg.paged_attention_prefill(q, s["k"], s["v"], s["table"], p.kv_lens, p.cu_tokens, window=50, sinks=2)
+    return a, b
+
+
+def test_a_run_of_steps(pkg):
+    """Steps on end, each against the 64-bit form on the cache as it then is; pages come in as lengths pass their end."""
+    s = step_state(1)
+    for i in range(20):
+        a, b = step(pkg, s)
+        lens, table = s["lens"].tolist(), s["table"].tolist()
+        assert lens == [38 + i, 1 + i, 301 + i, 65 + i]
+        q = oracle.norm_rope(s["qkv"][:, :16], s["w"], *(x.double()[[n - 1 for n in lens], :64] for x in (s["cos"], s["sin"])), 1e-6)
+        q = q.to(torch.bfloat16)
+        for out, window, sinks, rounded in ((a, 0, 0, False), (b, 50, 2, True)):
+            ref, mag = oracle.attend(q, s["k"], s["v"], table, [n - 1 for n in lens], 2, window, sinks, 128 ** -0.5)
+            # the kernels' queries were rounded from f32 sums, these from f64: a query now and then differs by a step, its
+            # scores (at most 4 at these norms) by 2^-8 of a channel's part: 1e-2 of the outputs' size in all
+            assert float((out.double() - ref).abs().max()) < 1e-2 * float(ref.abs().max()), (i, window)
+
+
+def test_captured_steps_replay_with_growing_lengths(pkg):
+    """A step captured once and replayed: lengths, pages and slots are read on the device, so every replay is the next
+    step. Eager steps of another batch and synchronizations go between the replays."""
+    s, e, other = step_state(2), step_state(2), step_state(3)
+    step(pkg, step_state(4), 400)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        a, b = step(pkg, s, 400)
+    for i in range(6):
+        g.replay()
+        want = step(pkg, e, 400)
+        step(pkg, other)
+        torch.cuda.synchronize()
+        assert s["lens"].tolist() == e["lens"].tolist() == [38 + i, 1 + i, 301 + i, 65 + i]
+        assert torch.equal(a, want[0]) and torch.equal(b, want[1]) and torch.equal(s["table"], e["table"])
+
+
+def test_two_streams_at_once(pkg):
+    """Two batches stepped on two streams at the same time, their split calls' workspaces apart: as one after the other."""
+    def batch(seed):
+        g = gen(seed)
+        lens = [3000, 700]
+        k, v, table = make_cache(g, lens, 64, 8, 128, torch.bfloat16)
+        return torch.randn(2, 16, 128, generator=g, device=DEV).to(torch.bfloat16), k, v, ints(table), ints(lens)
+    x, y = batch(1), batch(2)
+    want = [pkg.paged_attention_decode(*z) for z in (x, y)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, z in enumerate((x, y)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(pkg.paged_attention_decode(*z))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+def test_padded_batch_leaves_the_padding_alone(pkg):
+    """A captured size larger than the batch: tokens past the last request get slot -1 and store nothing; idle requests
+    (no new token, length 0 among them) attend what they hold."""
+    s = step_state(5)
+    k0, v0 = s["k"].clone(), s["v"].clone()
+    p = pkg.paged_plan(ints([0, 2, 0, 0]), s["lens"], s["table"], s["free"], s["count"], 16, 4)
+    assert p.slots.tolist()[2:] == [-1, -1] and p.kv_lens.tolist() == [37, 2, 300, 64] and p.cu_tokens.tolist() == [0, 0, 2, 2, 2]
+    q = torch.full((4, 16, 128), 3.0, dtype=torch.bfloat16, device=DEV)
+    x = s["qkv"]
+    out = pkg.qk_norm_rope_store(x[:, :16], x[:, 16:24], x[:, 24:], s["w"], s["w"], s["cos"], s["sin"], p.positions, p.slots, s["k"], s["v"], out=q)
+    assert bool((out[2:] == 3.0).all())
+    new = s["table"][1, 0].item()
+    keep = [i for i in range(k0.shape[0]) if i != new]
+    assert torch.equal(s["k"][keep].nan_to_num(9.0), k0[keep].nan_to_num(9.0)) and torch.equal(s["v"][keep].nan_to_num(9.0), v0[keep].nan_to_num(9.0))
+    o = torch.full((4, 16, 128), 5.0, dtype=torch.bfloat16, device=DEV)
+    pkg.paged_attention_prefill(q, s["k"], s["v"], s["table"], p.kv_lens, p.cu_tokens, out=o)
+    assert bool((o[2:] == 5.0).all()) and torch.isfinite(o).all() and not bool((o[:2] == 5.0).all())
