@@ -729,15 +729,15 @@ std::vector<Tensor> paged_plan(Tensor new_tokens, Tensor lengths, Tensor block_t
   TORCH_CHECK(block_table.size(1) <= INT_MAX / page_size, "a block_table row holds more than 2^31 - 1 tokens");
   int* len_out = lengths_out.has_value() ? const_cast<int*>(check_i32(*lengths_out, dev, n, "lengths_out")) : len;
   int* fc_out = free_count_out.has_value() ? const_cast<int*>(check_i32(*free_count_out, dev, 1, "free_count_out")) : fc;
-  auto i32 = torch::dtype(torch::kInt32).device(dev);
-  auto slots = torch::empty({total_tokens}, i32), positions = torch::empty({total_tokens}, i32);
-  auto cu = torch::empty({n + 1}, i32), kv = torch::empty({n}, i32), status = torch::empty({n}, i32);
+  auto parts = torch::empty({2 * total_tokens + 3 * n + 1}, torch::dtype(torch::kInt32).device(dev))
+                   .split_with_sizes({total_tokens, total_tokens, n + 1, n, n});
+  auto &slots = parts[0], &positions = parts[1], &cu = parts[2], &kv = parts[3], &status = parts[4];
   hip_check(qtts_paged_plan((int)n, (int)block_table.size(1), table_stride(block_table), (int)page_size, (int)total_tokens, nt, len,
                             block_table.data_ptr<int>(), fp, (int)std::min<int64_t>(free_pages.numel(), INT_MAX), fc,
                             slots.data_ptr<int>(), positions.data_ptr<int>(), cu.data_ptr<int>(), kv.data_ptr<int>(), len_out,
                             fc_out, status.data_ptr<int>(), cur_stream()),
             "qtts_paged_plan");
-  return {slots, positions, cu, kv, status};
+  return parts;
 }
 
 void paged_release(Tensor release, Tensor lengths, Tensor block_table, Tensor free_pages, Tensor free_count, int64_t page_size) {
