@@ -396,7 +396,9 @@ hipError_t qtts_paged_plan(int n_requests, int table_width, long long table_stri
   PlanArgs g{n_requests, table_width, __builtin_ctz((unsigned)page_size), total_tokens, table_stride, new_tokens, lengths,
              block_table, free_pages, free_capacity, free_count, slots, positions, cu_tokens, kv_lens, lengths_out,
              free_count_out, status, 0};
-  g.fill = total_tokens <= 8192;
+  // the tokens in the same launch while they are two for a thread; past that a second one over the whole GPU (us, one
+  // launch : two: 64 requests of one token 3.7 : 4.9, 200 of 10 9.3 : 6.8, 64 of 64 14.3 : 7.1, 60 of 700 113 : 12.8)
+  g.fill = total_tokens <= 2 * (n_requests <= 256 ? 256 : PT);
   if (n_requests <= 256) hipLaunchKernelGGL(plan_kernel<256>, dim3(1), dim3(256), 0, stream, g);
   else hipLaunchKernelGGL(plan_kernel<PT>, dim3(1), dim3(PT), 0, stream, g);
   if (!g.fill) hipLaunchKernelGGL(plan_tokens_kernel, dim3((unsigned)((total_tokens + 255) / 256)), dim3(256), 0, stream, g);
@@ -460,9 +462,11 @@ hipError_t qtts_qk_norm_rope_store(const QttsPagedCache* cache, int n_tokens, in
   g.w_end = w_channels;
   g.eps = eps;
   g.pages = pages_of(cache);
-  // a wave a token where the tokens alone fill the GPU, else a wave for each group of head rows
+  // a wave a token (its table row read once) from 2048 tokens on, 8 waves a CU; below, a wave for each group of head
+  // rows (us, a wave a token : a group, 16 / 8 heads of 128: 40 tokens 4.9 : 3.4, 1024 6.1 : 5.1, 2048 8.5 : 8.4,
+  // 3000 11.3 : 12.3, 6001 18.1 : 20.2)
   const int rpw = 1024 / cache->head_dim, groups = (num_q_heads + 2 * cache->num_kv_heads + rpw - 1) / rpw;
-  g.parts = n_tokens >= 4096 ? 1 : groups;
+  g.parts = n_tokens >= 2048 ? 1 : groups;
   if (((long long)n_tokens * g.parts + 3) / 4 > INT_MAX) return hipErrorInvalidValue;
   if (cache->dtype == QTTS_BF16) {
     if (cache->head_dim == 128) launch_store<Bf16, 128>(g, table_f32 != 0, stream);
