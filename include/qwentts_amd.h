@@ -366,7 +366,8 @@ typedef struct QttsPagedCache {
  * new_tokens[b] more (values below 0 count as 0); the tokens of all requests are packed in request
  * order into arrays of total_tokens. Pages are taken from the top of the stack free_pages[0 ..
  * *free_count) in request order; a request that finds too few ends the giving (none behind it
- * overtakes it). page_size is a power of two up to 65536.
+ * overtakes it). page_size is a power of two up to 65536, a table row holds up to 2^30 tokens, total_tokens is
+ * at most 2^30 and n_requests 2^24.
  *   block_table       gets the new pages of granted requests (other entries stay)
  *   slots, positions  [total_tokens]: slot and position of each token; -1 and the position it would
  *                     have where the request is refused, -1 and 0 past the last request's tokens
@@ -411,7 +412,8 @@ hipError_t qtts_qk_norm_rope_store(
  * softmax(scale q . k) v over the keys j < kv_lens[b]; with window > 0 only those with
  * j >= kv_lens[b] - window or j < sinks. Query head h reads KV head h / (num_q_heads /
  * num_kv_heads). A request of length 0 gets zeros, as does a query with no finite score; keys on
- * pages outside [0, num_pages) are not seen; lengths are clamped to [0, table_width * page_size].
+ * pages outside [0, num_pages) are not seen; lengths are clamped to
+ * [0, table_width * page_size], which is at most 2^30.
  * max_len: the longest request as far as the caller knows (it sets how the keys are split; longer
  * requests are computed too). scale > 0. The workspace of
  * qtts_paged_decode_workspace_bytes() bytes (0: none is used), 16-byte aligned, needs no

@@ -8,6 +8,7 @@
 // devices and positions are validated (the reference checks nothing), launch errors raise,
 // and extra methods expose the fused head / token-selection / frame entry points.
 #include <torch/extension.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <hip/hip_runtime_api.h>
@@ -661,6 +662,9 @@ void check_table(const Tensor& t, const torch::Device& dev, int64_t requests) {
   TORCH_CHECK(t.stride(1) == 1 || t.size(1) == 1, "block_table rows must be contiguous");
   TORCH_CHECK(t.size(0) == 1 || t.stride(0) >= t.size(1), "block_table rows must not overlap");
 }
+void check_capacity(const Tensor& t, int64_t page_size) {
+  TORCH_CHECK(t.size(1) <= (1ll << 30) / page_size, "a block_table row holds more than 2^30 tokens");
+}
 long long table_stride(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
 
 void check_page_size(int64_t page_size, int64_t least) {
@@ -718,15 +722,15 @@ std::vector<Tensor> paged_plan(Tensor new_tokens, Tensor lengths, Tensor block_t
   const torch::Device dev = new_tokens.device();
   c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
   const int64_t n = new_tokens.numel();
-  TORCH_CHECK(n >= 1 && n <= INT_MAX, "a plan needs at least one request");
-  TORCH_CHECK(total_tokens >= 0 && total_tokens <= INT_MAX, "total_tokens out of range: ", total_tokens);
+  TORCH_CHECK(n >= 1 && n <= (1 << 24), "a plan takes 1 .. 2^24 requests, got ", n);
+  TORCH_CHECK(total_tokens >= 0 && total_tokens <= (1 << 30), "total_tokens out of range: ", total_tokens);
   const int* nt = check_i32(new_tokens, dev, n, "new_tokens");
   int* len = const_cast<int*>(check_i32(lengths, dev, n, "lengths"));
   check_table(block_table, dev, n);
   const int* fp = check_i32(free_pages, dev, 0, "free_pages");
   int* fc = const_cast<int*>(check_i32(free_count, dev, 1, "free_count"));
   check_page_size(page_size, 1);
-  TORCH_CHECK(block_table.size(1) <= INT_MAX / page_size, "a block_table row holds more than 2^31 - 1 tokens");
+  check_capacity(block_table, page_size);
   int* len_out = lengths_out.has_value() ? const_cast<int*>(check_i32(*lengths_out, dev, n, "lengths_out")) : len;
   int* fc_out = free_count_out.has_value() ? const_cast<int*>(check_i32(*free_count_out, dev, 1, "free_count_out")) : fc;
   auto parts = torch::empty({2 * total_tokens + 3 * n + 1}, torch::dtype(torch::kInt32).device(dev))
@@ -745,7 +749,7 @@ void paged_release(Tensor release, Tensor lengths, Tensor block_table, Tensor fr
   const torch::Device dev = release.device();
   c10::hip::HIPGuardMasqueradingAsCUDA guard(dev);
   const int64_t n = release.numel();
-  TORCH_CHECK(n >= 1 && n <= INT_MAX, "a release needs at least one request");
+  TORCH_CHECK(n >= 1 && n <= (1 << 24), "a release takes 1 .. 2^24 requests, got ", n);
   const int* rel = check_i32(release, dev, n, "release");
   check_i32(lengths, dev, n, "lengths");
   check_table(block_table, dev, n);
@@ -804,10 +808,13 @@ Tensor qk_norm_rope_store(Tensor q, Tensor k, Tensor v, OptTensor q_weight, OptT
   if (out.has_value()) {
     o = *out;
     check_heads(o, k_cache, n, q.size(1), "out");
+    at::assert_no_internal_overlap(o);
   } else {
     o = torch::empty({n, q.size(1), dim}, q.options());
   }
   if (n == 0) return o;
+  at::assert_no_internal_overlap(k_cache);   // (an expanded cache: its rows are one)
+  at::assert_no_internal_overlap(v_cache);
   hip_check(qtts_qk_norm_rope_store(&cache, (int)n, (int)q.size(1), q.data_ptr(), tok_stride(q), head_stride(q), k.data_ptr(),
                                     tok_stride(k), head_stride(k), v.data_ptr(), tok_stride(v), head_stride(v), o.data_ptr(),
                                     tok_stride(o), head_stride(o), q_weight.has_value() ? q_weight->data_ptr() : nullptr,
@@ -828,12 +835,13 @@ Tensor check_attention(const QttsPagedCache& cache, const Tensor& q, const Tenso
   TORCH_CHECK(q.size(0) * q.size(1) <= INT_MAX / 2, "q has too many rows");
   TORCH_CHECK(requests >= 1 && requests <= INT_MAX, "at least one request is needed");
   check_table(block_table, dev, requests);
-  TORCH_CHECK(block_table.size(1) <= (INT_MAX - 4096) / cache.page_size, "a block_table row holds more than 2^31 - 4097 tokens");
+  check_capacity(block_table, cache.page_size);
   check_i32(kv_lens, dev, requests, "kv_lens");
   TORCH_CHECK(scale > 0.0 && std::isfinite((float)scale) && (float)scale > 0.0f, "scale must be positive and finite");
   TORCH_CHECK(window >= 0 && window <= INT_MAX && sinks >= 0 && sinks <= INT_MAX, "window and sinks must be >= 0");
   if (!out.has_value()) return torch::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   check_heads(*out, k_cache, q.size(0), q.size(1), "out");
+  at::assert_no_internal_overlap(*out);
   return *out;
 }
 
@@ -922,7 +930,7 @@ class PagedTTSBackbone {
     check_aligned(embeds, "embeds");
     TORCH_CHECK(cu_tokens.has_value() || tokens == n, "one token for each stream expected (", n, "), got ", tokens);
     check_table(block_table, dev_, n);
-    TORCH_CHECK(block_table.size(1) <= (INT_MAX - 4096) / cache.page_size, "a block_table row holds more than 2^31 - 4097 tokens");
+    check_capacity(block_table, cache.page_size);
     const int width = (int)block_table.size(1);
     TORCH_CHECK(max_len >= 1 && window >= 0 && window <= INT_MAX && sinks >= 0 && sinks <= INT_MAX, "max_len, window or sinks out of range");
     const int most = (int)std::min<int64_t>(max_len, (int64_t)width * cache.page_size);

@@ -385,10 +385,11 @@ hipError_t qtts_paged_plan(int n_requests, int table_width, long long table_stri
                            const int* new_tokens, const int* lengths, int* block_table, const int* free_pages,
                            int free_capacity, const int* free_count, int* slots, int* positions, int* cu_tokens,
                            int* kv_lens, int* lengths_out, int* free_count_out, int* status, hipStream_t stream) {
-  if (n_requests < 1 || table_width < 1 || table_stride < table_width || total_tokens < 0 || free_capacity < 0)
+  if (n_requests < 1 || n_requests > (1 << 24) || table_width < 1 || table_stride < table_width || total_tokens < 0 ||
+      total_tokens > (1 << 30) || free_capacity < 0)
     return hipErrorInvalidValue;
   if (page_size < 1 || page_size > 65536 || (page_size & (page_size - 1)) != 0) return hipErrorInvalidValue;
-  if ((long long)table_width * page_size > INT_MAX) return hipErrorInvalidValue;
+  if ((long long)table_width * page_size > (1ll << 30)) return hipErrorInvalidValue;
   if (new_tokens == nullptr || lengths == nullptr || block_table == nullptr || free_count == nullptr || cu_tokens == nullptr ||
       kv_lens == nullptr || lengths_out == nullptr || free_count_out == nullptr || status == nullptr ||
       (free_capacity > 0 && free_pages == nullptr) || (total_tokens > 0 && (slots == nullptr || positions == nullptr)))
@@ -408,7 +409,8 @@ hipError_t qtts_paged_plan(int n_requests, int table_width, long long table_stri
 hipError_t qtts_paged_release(int n_requests, int table_width, long long table_stride, int page_size, const int* release,
                               int* lengths, int* block_table, int* free_pages, int free_capacity, int* free_count,
                               hipStream_t stream) {
-  if (n_requests < 1 || table_width < 1 || table_stride < table_width || free_capacity < 1) return hipErrorInvalidValue;
+  if (n_requests < 1 || n_requests > (1 << 24) || table_width < 1 || table_stride < table_width || free_capacity < 1)
+    return hipErrorInvalidValue;
   if (page_size < 1 || page_size > 65536 || (page_size & (page_size - 1)) != 0) return hipErrorInvalidValue;
   if (release == nullptr || lengths == nullptr || block_table == nullptr || free_pages == nullptr || free_count == nullptr)
     return hipErrorInvalidValue;

@@ -283,12 +283,14 @@ __global__ void __launch_bounds__(64 * W, 2) decode_kernel(const AttnArgs g) {
       bm = fmaxf(bm, xlane_f<5>(bm));
       if (__builtin_amdgcn_ballot_w64(bm > m) != 0ull) {
         const float mn = fmaxf(m, bm);
-        const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * SL);
-        l *= al;
+        if (__builtin_amdgcn_ballot_w64(m > -INFINITY) != 0ull) {   // (else the sums are zeros)
+          const float al = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * SL);
+          l *= al;
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb)
+          for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[mb][r] *= al;
+            for (int r = 0; r < 4; ++r) o[mb][r] *= al;
+        }
         m = mn;
       }
       const float nm = m == -INFINITY ? 0.0f : -m * SL;
@@ -332,6 +334,52 @@ __global__ void __launch_bounds__(64 * W, 2) decode_kernel(const AttnArgs g) {
       }
       now = next;
     }
+  }
+  // A seen v_j that is infinite makes its channel's sum infinite, but 0 or a negative rest times it a NaN. Sums that are
+  // not finite are taken again in 32 bits, key by key. (The rests in sums of their own, dropped there, were 3% slower.)
+  float odd = 0.0f;
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) odd = fmaf(o[mb][r], 0.0f, odd);
+  if (__builtin_amdgcn_ballot_w64(odd != 0.0f) != 0ull) {
+    f32x4 again[MB];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) again[mb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const float nm = m == -INFINITY ? 0.0f : -m * SL;
+#pragma unroll 1
+    for (int i = 0; i < nt; ++i) {
+      const Block x = block(entries(i), i);
+#pragma unroll 1
+      for (int j = 0; j < DKB; ++j) {
+        const int key = x.key0 + j, u = j >> 4;
+        if (!sees(x, key, u)) continue;
+        const long long at = (long long)(u ? x.page[1] : x.page[0]) * g.pages.page_stride +
+                             (long long)(key & ((1 << g.pages.shift) - 1)) * g.pages.slot_stride;
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const u32x4 kk = ldw(k_head + at + 32 * k + 8 * gr);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) s = fmaf(E::lo(q[k][h]), E::lo(kk[h]), fmaf(E::hi(q[k][h]), E::hi(kk[h]), s));
+        }
+        s += xlane_f<4>(s);
+        s += xlane_f<5>(s);
+        const float p = __builtin_amdgcn_exp2f(fmaf(s, SL, nm));
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          const u32x2 v = *gmem(reinterpret_cast<const u32x2*>(v_head + at + 16 * mb + 4 * gr));
+          again[mb][0] = fmaf(p, E::lo(v[0]), again[mb][0]);
+          again[mb][1] = fmaf(p, E::hi(v[0]), again[mb][1]);
+          again[mb][2] = fmaf(p, E::lo(v[1]), again[mb][2]);
+          again[mb][3] = fmaf(p, E::hi(v[1]), again[mb][3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[mb][r] = (__float_as_uint(o[mb][r]) & 0x7fffffffu) < 0x7f800000u ? o[mb][r] : again[mb][r];
   }
   l += xlane_f<4>(l);
   l += xlane_f<5>(l);
@@ -909,6 +957,8 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
 
 // ---- host ----------------------------------------------------------------------------------
 
+constexpr long long kMostKeys = 1ll << 30;   // of a table row: positions and windows stay inside int
+
 bool attn_ok(const QttsPagedCache* cache, int n_tokens, int hq, const void* q, long long q_token, long long q_head, const void* out,
              long long o_token, long long o_head, const int* table, int width, long long table_stride, const int* lens,
              int requests, float scale, int window, int sinks) {
@@ -916,7 +966,7 @@ bool attn_ok(const QttsPagedCache* cache, int n_tokens, int hq, const void* q, l
   if (q == nullptr || out == nullptr || table == nullptr || lens == nullptr) return false;
   if (((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out)) & 15u) != 0) return false;
   if (((q_token | q_head | o_token | o_head) & 7) != 0) return false;
-  if (width < 1 || table_stride < width || (long long)width * cache->page_size > INT_MAX - 4096) return false;
+  if (width < 1 || table_stride < width || (long long)width * cache->page_size > kMostKeys) return false;
   if (!(scale > 0.0f) || !std::isfinite(scale) || window < 0 || sinks < 0) return false;
   return (long long)n_tokens * hq <= INT_MAX / 2;
 }
@@ -938,7 +988,7 @@ AttnArgs attn_args(const QttsPagedCache* cache, int hq, const void* q, long long
   g.group = hq / cache->num_kv_heads;
   g.hkv = cache->num_kv_heads;
   g.scale_log2 = scale * 1.4426950408889634f;
-  g.window = window;
+  g.window = (int)std::min<long long>(window, kMostKeys);   // (as good as none)
   g.sinks = window > 0 ? sinks : 0;
   return g;
 }

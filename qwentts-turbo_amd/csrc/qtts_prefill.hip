@@ -41,6 +41,7 @@
 #include <cstdint>
 #include "qwentts_amd.h"
 #include "qtts_common.h"
+#include "qtts_paged.h"
 #include "qtts_select.h"
 
 namespace qtts {
@@ -1458,7 +1459,8 @@ size_t qtts_paged_workspace_bytes(int n_tokens, int n_requests, int vocab, int t
 }
 
 hipError_t qtts_backbone_paged(void* workspace, size_t workspace_bytes, const TTSLayerWeights* layer_weights,
-                               const TTSLayerWeights* host_layers, int num_layers, const void* final_norm_weight, const void* cos_table, const void* sin_table, int table_rows,
+                               const TTSLayerWeights* host_layers, int num_layers, const void* final_norm_weight,
+                               const void* cos_table, const void* sin_table, int table_rows,
                                const QttsPagedCache* cache, long long layer_stride, int n_requests, int n_tokens,
                                const int* slots, const int* positions, const int* cu_tokens, const int* kv_lens,
                                const int* block_table, int table_width, long long table_stride, int max_len, int window,
@@ -1473,7 +1475,9 @@ hipError_t qtts_backbone_paged(void* workspace, size_t workspace_bytes, const TT
   if (num_layers < 1 || n_requests < 1 || n_tokens < 1 || n_tokens > (1 << 20) || n_requests > 65535 * HRB || table_rows < 1 || max_len < 1 || window < 0 ||
       sinks < 0 || layer_stride < 0 || (layer_stride & 7) != 0)
     return hipErrorInvalidValue;
-  if (cache->dtype != QTTS_BF16 || cache->num_kv_heads != NKVH || cache->head_dim != HDIM || table_width < 1 || cache->page_size < 16)
+  if (!pg::cache_ok(cache) || cache->dtype != QTTS_BF16 || cache->num_kv_heads != NKVH || cache->head_dim != HDIM)
+    return hipErrorInvalidValue;
+  if (table_width < 1 || table_stride < table_width || (long long)table_width * cache->page_size > (1ll << 30))
     return hipErrorInvalidValue;
   if (cu_tokens == nullptr && n_tokens != n_requests) return hipErrorInvalidValue;   // (one token each, in order)
   if (codec_head != nullptr && (vocab < 128 || vocab > MAXV || vocab % 128 != 0 || out_tokens == nullptr)) return hipErrorInvalidValue;

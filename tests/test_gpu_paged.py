@@ -208,7 +208,7 @@ HEADS = [(16, 8, 128), (4, 4, 64), (9, 3, 128), (20, 1, 64), (16, 1, 128), (40, 
 
 @pytest.mark.parametrize("hq,hkv,dim", HEADS)
 @pytest.mark.parametrize("dtype,page,layout", [(torch.bfloat16, 16, "heads_first"), (torch.float16, 64, "tokens_first")])
-@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (37, 3), (300, 50)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (37, 3), (300, 50), (2 ** 31 - 1, 2 ** 31 - 1)])
 def test_decode(pkg, hq, hkv, dim, dtype, page, layout, window, sinks):
     lens = [0, 1, 15, 16, 17, 31, 32, 33, 64, 129, 511, 640, 1025, 2100]
     g = gen(hq * dim + window)
@@ -226,7 +226,7 @@ PROMPTS = [(0, 1), (0, 0), (5, 1), (0, 63), (0, 64), (1, 65), (40, 30), (100, 0)
 
 @pytest.mark.parametrize("hq,hkv,dim", HEADS)
 @pytest.mark.parametrize("dtype,page,layout", [(torch.bfloat16, 16, "heads_first"), (torch.float16, 64, "tokens_first")])
-@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (37, 3), (100, 70)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (37, 3), (100, 70), (2 ** 31 - 1, 5)])
 def test_prefill(pkg, hq, hkv, dim, dtype, page, layout, window, sinks):
     run_prefill(pkg, PROMPTS, hq, hkv, dim, dtype, page, layout, window, sinks)
 
@@ -315,6 +315,29 @@ def test_hidden_keys_that_are_not_finite(pkg, bad):
     one = pkg.paged_attention_decode(q[:1], k, v, ints(table), ints([66]), window=15)
     r1, m1 = oracle.attend(q[:1], k, v, table, [65], 2, 15, 0, 128 ** -0.5)
     check(one, r1, m1, torch.bfloat16, False)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_infinite_values_that_are_seen(pkg, dtype, dim):
+    """A visible infinite V makes its channels infinite (both signs: NaN) and leaves the other channels alone."""
+    g = gen(12)
+    lens = [700, 40]
+    k, v, table = make_cache(g, lens, 16, 2, dim, dtype)
+    inf = float("inf")
+    for r, at, d, x in ((0, 650, 3, inf), (0, 20, 5, -inf), (0, 30, 7, inf), (0, 500, 7, -inf), (1, 39, 1, inf)):
+        v[table[r][at // 16], :, at % 16, d] = x
+    q = (0.2 * torch.randn(2, 4, dim, generator=g, device=DEV)).to(dtype)   # weights of 1e-3 and more: none rounds to 0
+    ref, mag = oracle.attend(q, k, v, table, [n - 1 for n in lens], 2, 0, 0, dim ** -0.5)
+    one = pkg.paged_attention_decode(q, k, v, ints(table), ints(lens))
+    two = pkg.paged_attention_prefill(q, k, v, ints(table), ints(lens), ints([0, 1, 2]))
+    fin = torch.isfinite(ref)
+    assert int((~fin).sum()) == 4 * 3 + 4
+    for out in (one, two):
+        o = out.double()
+        assert torch.equal(torch.isfinite(o), fin) and torch.equal(torch.isnan(o), torch.isnan(ref))
+        assert torch.equal(o[~fin & ~torch.isnan(ref)], ref[~fin & ~torch.isnan(ref)])
+        h = half(dtype)
+        assert bool(((o - ref).abs() <= 1.01 * h * ref.abs() + (3e-4 + h) * mag)[fin].all())
 
 
 def test_large_scores_and_scale(pkg):
@@ -443,6 +466,12 @@ def test_refusals(pkg):
         a.update(bad)
         with pytest.raises(RuntimeError):
             pkg.paged_plan(**a)
+    for bad in (dict(out=q[:1].expand(3, 16, 128)), dict(out=q[:, :1].expand(3, 16, 128))):
+        for call in (decode, prefill, store):
+            with pytest.raises(RuntimeError, match="overlap|single memory"):
+                call(**bad)
+    with pytest.raises(RuntimeError, match="overlap|single memory"):
+        store(k_cache=k[:1].expand(4, 8, 16, 128), v_cache=v[:1].expand(4, 8, 16, 128))
     assert bool((k == 0).all()) and bool((v == 0).all())
     assert store().shape == (3, 16, 128) and decode().shape == (3, 16, 128)
 

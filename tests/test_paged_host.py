@@ -14,18 +14,15 @@ P, I, L, F, Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 INVALID = 1                       # hipErrorInvalidValue
 A = 1 << 20                       # an aligned address that nothing reads
 
-
 class Cache(ctypes.Structure):
     _fields_ = [("k", P), ("v", P), ("dtype", I), ("num_pages", I), ("page_size", I), ("num_kv_heads", I), ("head_dim", I),
                 ("page_stride", L), ("head_stride", L), ("slot_stride", L)]
-
 
 def cache(**kw):
     d = dict(k=A, v=A, dtype=0, num_pages=4, page_size=16, num_kv_heads=8, head_dim=128, page_stride=8 * 16 * 128,
              head_stride=16 * 128, slot_stride=128)
     d.update(kw)
     return Cache(**d)
-
 
 @pytest.fixture(scope="module")
 def lib():
@@ -39,16 +36,16 @@ def lib():
     x.qtts_paged_attention_prefill.argtypes = [P, I, I, I, P, L, L, P, L, L, P, I, L, P, P, I, F, I, I, P]
     x.qtts_paged_decode_workspace_bytes.argtypes = [I] * 9
     x.qtts_paged_decode_workspace_bytes.restype = Z
+    x.qtts_backbone_paged.argtypes = [P, Z, P, P, I, P, P, P, I, P, L, I, I, P, P, P, P, P, I, L, I, I, I, P, P, P, I, P, P, I, P, I, P, I, F,
+                                      I, I, P, I, P, P]
     x.qtts_paged_workspace_bytes.argtypes = [I] * 8
     x.qtts_paged_workspace_bytes.restype = Z
     return x
-
 
 BAD_CACHES = [dict(k=0), dict(v=0), dict(k=A + 8), dict(v=A + 2), dict(dtype=2), dict(dtype=-1), dict(num_pages=0), dict(num_kv_heads=0),
               dict(head_dim=96), dict(head_dim=256), dict(page_size=8), dict(page_size=48), dict(page_size=0), dict(page_size=1 << 17),
               dict(page_stride=1004), dict(page_stride=-8), dict(page_stride=1 << 31), dict(head_stride=4), dict(head_stride=1 << 31),
               dict(slot_stride=64), dict(slot_stride=132), dict(slot_stride=(1 << 24) + 8)]
-
 
 def store(lib, c=None, **kw):
     d = dict(n=3, hq=16, q=A, qt=2048, qh=128, k=A, kt=1024, kh=128, v=A, vt=1024, vh=128, o=A, ot=2048, oh=128, wq=A, wk=A, eps=1e-6,
@@ -56,13 +53,11 @@ def store(lib, c=None, **kw):
     d.update(kw)
     return lib.qtts_qk_norm_rope_store(ctypes.byref(c) if c is not None else None, *d.values(), None)
 
-
 def decode(lib, c=None, **kw):
     d = dict(n=3, hq=16, q=A, qt=2048, qh=128, o=A, ot=2048, oh=128, table=A, width=4, stride=4, lens=A, max_len=64, scale=0.1, window=0,
              sinks=0, ws=A, wsb=1 << 30)
     d.update(kw)
     return lib.qtts_paged_attention_decode(ctypes.byref(c) if c is not None else None, *d.values(), None)
-
 
 def prefill(lib, c=None, **kw):
     d = dict(n=3, t=9, hq=16, q=A, qt=2048, qh=128, o=A, ot=2048, oh=128, table=A, width=4, stride=4, lens=A, cu=A, max_len=64, scale=0.1,
@@ -70,12 +65,10 @@ def prefill(lib, c=None, **kw):
     d.update(kw)
     return lib.qtts_paged_attention_prefill(ctypes.byref(c) if c is not None else None, *d.values(), None)
 
-
 @pytest.mark.parametrize("bad", BAD_CACHES, ids=str)
 def test_caches_that_kernels_cannot_address(lib, bad):
     for call in (store, decode, prefill):
         assert call(lib, cache(**bad)) == INVALID, call.__name__
-
 
 def test_store_refusals(lib):
     c = cache()
@@ -86,12 +79,11 @@ def test_store_refusals(lib):
         assert store(lib, c, **bad) == INVALID, bad
     assert store(lib, c, n=0) == 0                                          # nothing to do, nothing launched
 
-
 def test_attention_refusals(lib):
     c = cache()
     assert decode(lib) == INVALID and prefill(lib) == INVALID
     for bad in (dict(n=0), dict(hq=0), dict(hq=12), dict(q=0), dict(o=0), dict(table=0), dict(lens=0), dict(q=A + 2), dict(o=A + 8),
-                dict(qt=3), dict(oh=4), dict(width=0), dict(stride=3), dict(width=1 << 27, stride=1 << 27), dict(max_len=0), dict(scale=0.0),
+                dict(qt=3), dict(oh=4), dict(width=0), dict(stride=3), dict(width=(1 << 26) + 1, stride=1 << 27), dict(max_len=0), dict(scale=0.0),
                 dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(window=-1), dict(sinks=-1)):
         assert decode(lib, c, **bad) == INVALID, bad
         assert prefill(lib, c, **bad) == INVALID, bad
@@ -103,7 +95,6 @@ def test_attention_refusals(lib):
     for bad in (dict(ws=0), dict(wsb=need - 1), dict(ws=A + 8)):
         assert decode(lib, c, **big, **bad) == INVALID, bad
 
-
 def test_plan_and_release_refusals(lib):
     def plan(**kw):
         d = dict(n=2, width=4, stride=4, page=16, total=8, new=A, len=A, table=A, free=A, cap=9, count=A, slots=A, pos=A, cu=A, kv=A, lo=A,
@@ -111,7 +102,7 @@ def test_plan_and_release_refusals(lib):
         d.update(kw)
         return lib.qtts_paged_plan(*d.values(), None)
     for bad in (dict(n=0), dict(width=0), dict(stride=3), dict(page=0), dict(page=24), dict(page=1 << 17), dict(total=-1), dict(cap=-1),
-                dict(width=1 << 20, stride=1 << 20, page=1 << 16), dict(free=0), *(dict([(k, 0)]) for k in
+                dict(width=(1 << 14) + 1, stride=1 << 20, page=1 << 16), dict(free=0), dict(total=(1 << 30) + 1), dict(n=(1 << 24) + 1), *(dict([(k, 0)]) for k in
                 ("new", "len", "table", "count", "slots", "pos", "cu", "kv", "lo", "fo", "st"))):
         assert plan(**bad) == INVALID, bad
 
@@ -123,6 +114,25 @@ def test_plan_and_release_refusals(lib):
                 ("rel", "len", "table", "free", "count"))):
         assert release(**bad) == INVALID, bad
 
+def test_backbone_refusals(lib):
+    need = lib.qtts_paged_workspace_bytes(3, 3, 256, 4, 16, 64, 0, 0)
+    assert need > 0
+
+    def run(c, **kw):
+        d = dict(ws=A, wsb=need, layers=A, host=A, nl=2, norm=A, cos=A, sin=A, rows=64, cache=ctypes.byref(c) if c is not None else None,
+                 ls=0, n=3, t=3, slots=A, pos=A, cu=0, kv=A, table=A, width=4, stride=4, max_len=64, window=0, sinks=0, x=A, hidden=A,
+                 head=A, vocab=256, logits=0, tokens=A, mask=0, hist=0, hs=0, nh=0, hl=0, rep=1.0, eos=-1, sup=0, sampling=0, frame=0,
+                 skip=0)
+        d.update(kw)
+        return lib.qtts_backbone_paged(*d.values(), None)
+    for bad in BAD_CACHES + [dict(dtype=1), dict(num_kv_heads=4), dict(head_dim=64, slot_stride=64)]:
+        assert run(cache(**bad)) == INVALID, bad
+    assert run(None) == INVALID
+    for bad in (*(dict([(k, 0)]) for k in ("ws", "layers", "host", "nl", "norm", "cos", "sin", "rows", "n", "t", "slots", "pos", "kv", "table",
+                                           "width", "max_len", "x", "hidden", "tokens")),
+                dict(ws=A + 128), dict(wsb=need - 1), dict(ls=-8), dict(ls=4), dict(t=4), dict(t=(1 << 20) + 1, cu=A), dict(stride=3),
+                dict(width=(1 << 26) + 1, stride=1 << 27), dict(window=-1), dict(sinks=-1), dict(x=A + 2), dict(vocab=100), dict(vocab=8192)):
+        assert run(cache(), **bad) == INVALID, bad
 
 def test_workspace_queries(lib):
     f, g = lib.qtts_paged_decode_workspace_bytes, lib.qtts_paged_workspace_bytes
@@ -133,7 +143,6 @@ def test_workspace_queries(lib):
     assert f(1, 16, 8, 128, 4096, 16, 65536, 100, 4) < one                  # a window bounds the units
     assert g(0, 1, 0, 4, 16, 9, 0, 0) == 0 and g(1, 1, 3073, 4, 16, 9, 0, 0) == 0
     assert 0 < g(1, 1, 0, 4, 16, 9, 0, 0) < g(64, 64, 3072, 4, 16, 9, 0, 0)
-
 
 def test_python_functions_refuse_host_tensors(pkg):
     z = torch.zeros(4, dtype=torch.int32)
@@ -147,7 +156,6 @@ def test_python_functions_refuse_host_tensors(pkg):
         with pytest.raises(RuntimeError, match="GPU tensor"):
             call()
 
-
 def test_oracle_plan_by_hand():
     """The plan's oracle on a case worked out by hand: pages of 4, stack [7, 8, 9] with 9 on top."""
     table = [[5, -1, -1], [-1, -1, -1], [6, -1, -1]]
@@ -155,7 +163,6 @@ def test_oracle_plan_by_hand():
     assert table == [[5, 9, -1], [8, 7, -1], [6, -1, -1]]
     assert r == dict(slots=[23, 36, 32, 33, 34, 35, 28, -1], positions=[3, 4, 0, 1, 2, 3, 4, 4], cu=[0, 2, 7, 8], kv=[5, 5, 0],
                      held=[5, 5, 4], status=[0, 0, 1], count=0)
-
 
 def test_oracle_attention_against_a_dense_softmax():
     g = torch.Generator().manual_seed(1)
