@@ -92,7 +92,8 @@ class BatchedTTSDecoder:
         whose ``skip[s]`` is nonzero computes nothing, writes no KV entry and leaves its token,
         logits and residual as they were, but its position still advances (the host does not
         read the flag, so no launch waits on the device), so its cache holds an unwritten slot
-        and the stream must not be resumed. Its row of the returned hiddens is zero. Returns the
+        and the stream must not be resumed (``paged``: no page is taken for it). Its row of the
+        returned hiddens is zero. Returns the
         final-norm hiddens (f32 [n_streams, 1024], device)."""
         if skip is not None and (skip.dtype != torch.int32 or skip.numel() != self.n_streams or not skip.is_contiguous()):
             raise ValueError("skip must be a contiguous device int32 tensor with one entry per stream")

@@ -147,12 +147,18 @@ class PagedBackbone:
         paged_release(mask, self.lengths, self.block_table, self.free_pages, self.free_count, self.page_size)
         self.failed.masked_fill_(mask != 0, 0)
 
-    def _plan(self, counts: Sequence[int]) -> PagedPlan:
+    def _plan(self, counts: Sequence[int], off: Optional[torch.Tensor] = None) -> PagedPlan:
+        """``counts[s]`` more tokens of every stream s; none for those that the mask ``off`` marks."""
+        if len(counts) != self.n_streams or any(n < 0 for n in counts):
+            raise ValueError(f"counts must hold a number of tokens for each of {self.n_streams} streams, got {list(counts)}")
         for s, n in enumerate(counts):
             if self.positions[s] + n > self.max_seq_len:
                 raise RuntimeError(f"stream {s}: position {self.positions[s]} + {n} tokens exceeds max_seq_len {self.max_seq_len} "
                                    "(KV cache full)")
-        new = self._ones if all(n == 1 for n in counts) else torch.tensor(list(counts), dtype=torch.int32, device=self.device)
+        if off is not None:
+            new = (~off).to(torch.int32)
+        else:
+            new = self._ones if all(n == 1 for n in counts) else torch.tensor(list(counts), dtype=torch.int32, device=self.device)
         plan = paged_plan(new, self.lengths, self.block_table, self.free_pages, self.free_count, self.page_size, sum(counts))
         torch.maximum(self.failed, plan.status, out=self.failed)
         for s, n in enumerate(counts):
@@ -169,6 +175,7 @@ class PagedBackbone:
         counts[stream] = int(k.shape[2])
         slots = self._plan(counts).slots.long()
         if not bool((slots >= 0).all()):
+            self.reset([stream])
             raise RuntimeError(f"stream {stream}: the pool has too few free pages for {counts[stream]} tokens")
         page, place = slots // self.page_size, slots % self.page_size
         for pool, x in ((self.k_pool, k), (self.v_pool, v)):
@@ -183,14 +190,25 @@ class PagedBackbone:
         single = all(n == 1 for n in counts)
         if skip is not None and not single:
             raise ValueError("skip needs one token for every stream")
-        if embeds.shape != (sum(counts), HIDDEN_SIZE):
-            raise ValueError(f"embeds must be [{sum(counts)}, {HIDDEN_SIZE}], got {tuple(embeds.shape)}")
-        plan = self._plan(counts)
-        slots, lens = plan.slots, plan.kv_lens
-        if skip is not None:            # a finished stream stores and attends nothing
-            slots = torch.where(skip != 0, -1, slots)
-            lens = torch.where(skip != 0, 0, lens)
-        return self.kernel.forward(embeds, self.k_pool, self.v_pool, self.block_table, slots, plan.positions,
+        if embeds.shape != (sum(counts), HIDDEN_SIZE) or sum(counts) < 1:
+            raise ValueError(f"embeds must be [{sum(counts)}, {HIDDEN_SIZE}] with at least one token, got {tuple(embeds.shape)}")
+        # whatever the call refuses, it refuses before a page is taken
+        embeds = embeds.to(self.device, torch.bfloat16).contiguous()
+        for name, x, size in (("out_tokens", out_tokens, self.n_streams), ("skip", skip, self.n_streams),
+                              ("history", select.get("history"), 0), ("n_history", select.get("n_history"), self.n_streams)):
+            if x is not None and (x.dtype != torch.int32 or x.device != self.lengths.device or not x.is_contiguous() or x.numel() < size):
+                raise ValueError(f"{name} must be a contiguous int32 tensor on {self.lengths.device} with an entry for each stream")
+        if select.get("do_sample") and not select.get("temperature", 1.0) > 0:
+            raise ValueError("temperature must be > 0")
+        off = skip[:self.n_streams] != 0 if skip is not None else None
+        plan = self._plan(counts, off)
+        slots, positions, lens = plan.slots, plan.positions, plan.kv_lens
+        if off is not None:             # a finished stream takes no page, stores and attends nothing; rows stay in stream order
+            first = plan.cu_tokens[:-1]
+            slots = torch.where(off, -1, slots.index_select(0, first))
+            positions = positions.index_select(0, first)
+            lens = torch.where(off, 0, lens)
+        return self.kernel.forward(embeds, self.k_pool, self.v_pool, self.block_table, slots, positions,
                                    None if single else plan.cu_tokens, lens, max(self.positions), self.window, self.sinks,
                                    out_tokens=out_tokens, skip=skip, **select)
 

@@ -106,7 +106,8 @@ def test_selection_matches_the_oracle_sampler(pkg, model, sample):
         lg = apply_repetition_penalty(lg, [i for i in hist[s, :nh[s]].tolist() if 0 <= i < 3072], 1.3)
         lg[suppress_mask(3072, EOS)] = float("-inf")
         assert int(tok[s]) == sample_token(lg, sample, 0.9, 50, 0.9, EOS, seed=31 + s, frame_step=4, group=0)
-    assert dec.paged.lengths.tolist() == [1] * n               # skipped streams' positions advance all the same
+    # skipped streams' positions advance all the same, but they hold nothing for it
+    assert dec.positions() == [1] * n and dec.paged.lengths.tolist() == (1 - skip).tolist()
 
 
 @pytest.mark.parametrize("sample", [False, True], ids=["greedy", "sampled"])
@@ -166,6 +167,48 @@ def test_pool_runs_out_and_is_reset(pkg, model):
     h = dec.paged.forward(rows(3, 1 + 8 + 8).cuda(), [1, 8, 8])
     dec.check_error()
     assert torch.isfinite(h).all() and dec.positions() == [34, 8, 8]
+
+
+def test_finished_streams_take_no_pages(pkg, model):
+    """Steps with ``skip``: the pool's last pages go to the streams that go on, whose results are those of a decoder
+    without the finished ones; a finished stream is no failure."""
+    dsd, _ = model
+    make = lambda n, pages: pkg.BatchedTTSDecoder(dsd, n, max_seq_len=64, mode="paged", page_size=16, num_pages=pages)
+    dec, alone = make(4, 6), make(2, 4)
+    x = rows(1, 64).cuda()
+    dec.paged.forward(x, [16] * 4)
+    alone.paged.forward(torch.cat((x[16:32], x[48:])), [16, 16])
+    skip = torch.tensor([1, 0, 1, 0], dtype=torch.int32, device="cuda")
+    tok, tok2 = torch.full((4,), -7, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    for i in range(3):
+        y = rows(5 + i, 4).cuda()
+        h = dec.step_select(y, tok, EOS, skip=skip)
+        h2 = alone.step_select(y[1::2].contiguous(), tok2, EOS)
+        assert torch.equal(h[1::2], h2) and bool((h[::2] == 0).all())
+        assert torch.equal(tok[1::2], tok2) and tok[::2].tolist() == [-7, -7]
+    dec.check_error()
+    assert dec.paged.lengths.tolist() == [16, 19, 16, 19] and dec.paged.free_count.item() == 0
+
+
+def test_refused_calls_leave_the_pool_as_it_was(pkg, model):
+    dsd, _ = model
+    dec = pkg.BatchedTTSDecoder(dsd, 2, max_seq_len=64, mode="paged", page_size=16, num_pages=3)
+    x, ok = rows(1, 2).cuda(), torch.zeros(2, dtype=torch.int32, device="cuda")
+    for call in (lambda: dec.step_select(x, ok.cpu(), EOS), lambda: dec.step_select(x, torch.zeros(2, 2, dtype=torch.int32, device="cuda")[:, 0], EOS),
+                 lambda: dec.step_select(x, ok, EOS, skip=ok.cpu()), lambda: dec.step_select(x, ok, EOS, do_sample=True, temperature=0.0),
+                 lambda: dec.paged.forward(x, [1]), lambda: dec.paged.forward(x, [3, -1]), lambda: dec.paged.forward(x[:0], [0, 0])):
+        with pytest.raises(ValueError):
+            call()
+    k = torch.zeros(2, 8, 64, 128)
+    with pytest.raises(RuntimeError, match="free pages"):
+        dec.set_kv_cache(1, k, k)
+    assert dec.positions() == [0, 0] and dec.paged.lengths.tolist() == [0, 0] and dec.paged.free_count.item() == 3
+    dec.check_error()
+    # other types and strides of embeddings are taken as they are
+    a = dec.paged.forward(x, [1, 1])
+    dec.paged.reset()
+    b = dec.paged.forward(x.float().t().contiguous().t(), [1, 1])
+    assert torch.equal(a, b)
 
 
 def test_refusals(pkg, model):
