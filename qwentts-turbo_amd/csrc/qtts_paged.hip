@@ -136,8 +136,9 @@ __global__ void __launch_bounds__(NT) plan_kernel(const PlanArgs g) {
     const int m = min(NT, g.n - base);
     // pages given: the last sum that the free ones cover
     if (t < m && taken <= free_n && (t + 1 == m || s_taken[t + 1] > free_n)) s_given = taken;
-    // new pages: page q of the chunk's, asked by request r
-    for (long long q = t; q < sum_taken; q += NT) {
+    // new pages: page q of the chunk's that the free ones cover, asked by request r
+    const long long most = min(sum_taken, free_n - carry_taken);
+    for (long long q = t; q < most; q += NT) {
       const int r = first_above(s_taken, m, carry_taken + q);
       if (s_have[r] < 0) continue;
       const long long at = s_have[r] + carry_taken + q - (r ? s_taken[r - 1] : carry_taken);

@@ -336,13 +336,16 @@ __global__ void __launch_bounds__(64 * W, 2) decode_kernel(const AttnArgs g) {
     }
   }
   // A seen v_j that is infinite makes its channel's sum infinite, but 0 or a negative rest times it a NaN. Sums that are
-  // not finite are taken again in 32 bits, key by key. (The rests in sums of their own, dropped there, were 3% slower.)
+  // not finite are taken again in 32 bits, key by key (a sum of weights that is NaN makes NaN of them anyway). The rests
+  // in sums of their own, dropped there, were 3% slower.
+  l += xlane_f<4>(l);
+  l += xlane_f<5>(l);
   float odd = 0.0f;
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
     for (int r = 0; r < 4; ++r) odd = fmaf(o[mb][r], 0.0f, odd);
-  if (__builtin_amdgcn_ballot_w64(odd != 0.0f) != 0ull) {
+  if (__builtin_amdgcn_ballot_w64((odd != 0.0f) & (l == l)) != 0ull) {
     f32x4 again[MB];
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) again[mb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -381,8 +384,6 @@ __global__ void __launch_bounds__(64 * W, 2) decode_kernel(const AttnArgs g) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) o[mb][r] = (__float_as_uint(o[mb][r]) & 0x7fffffffu) < 0x7f800000u ? o[mb][r] : again[mb][r];
   }
-  l += xlane_f<4>(l);
-  l += xlane_f<5>(l);
 
   // join the waves: M = max m_w, L = sum l_w e^(m_w - M), O = sum O_w e^(m_w - M)
   static_assert(D * 16 * 4 <= 2 * BLK, "the join's sums");
@@ -520,7 +521,7 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const AttnArgs g) {
 // splits of a row join through LDS in key order.
 // A weight that is masked is 0, but 0 times an infinite or NaN v_j is NaN, and a key may be hidden from one
 // row of a tile and seen by another: rows that end with a number that is not finite are summed again over
-// the keys that they see, one by one (exact_row).
+// the keys that they see, one by one (exact_row); not those whose sum of weights is NaN: a score that they see is.
 constexpr int PWV = 8;                // waves
 
 // Row `r` of (request b, KV head kvh) again, key by key: the wave's lanes take D / 64 channels each.
@@ -935,7 +936,8 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
 #pragma unroll
     for (int v = 0; v < NS; ++v) worst = max(worst, __float_as_uint(sml[2 * v * 32 + c]));
   }
-  if (stored && worst < 0x7f800000u) {
+  const bool redo = (worst >= 0x7f800000u) & (L == L);
+  if (stored && !redo) {
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
       const int e = ks * NQ + j;
@@ -945,7 +947,7 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
       *reinterpret_cast<u32x2*>(op + 8 * e) = p;
     }
   }
-  uint64_t again = __builtin_amdgcn_ballot_w64(stored && worst >= 0x7f800000u) & 0xffffffffull;
+  uint64_t again = __builtin_amdgcn_ballot_w64(stored & redo) & 0xffffffffull;
   for (int n = 0; again != 0ull; ++n) {        // the splits take them in turn
     const int src = __builtin_ctzll(again);
     again &= again - 1;

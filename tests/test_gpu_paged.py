@@ -248,6 +248,41 @@ def run_prefill(pkg, prompts, hq, hkv, dim, dtype, page, layout, window, sinks, 
     return got
 
 
+@pytest.mark.parametrize("hq,hkv,dim", [(40, 2, 128), (80, 2, 64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 40)])
+@pytest.mark.parametrize("max_len", [1, 200, 700])
+def test_prefill_tiles(pkg, hq, hkv, dim, dtype, window, sinks, max_len):
+    """What the host says of the longest request chooses the tile: 1 the rows unsplit, 200 two key splits, 700 four (two
+    under the window). Nothing that is computed depends on it."""
+    run_prefill(pkg, PROMPTS, hq, hkv, dim, dtype, 32, "heads_first", window, sinks, max_len=max_len)
+
+
+@pytest.mark.parametrize("max_len", [1, 200, 700])
+def test_not_finite_in_each_tile(pkg, max_len):
+    """Per tile: an infinite V that half of the rows see, queries that are NaN; the other rows and requests as they were."""
+    g = gen(31)
+    prompts = PROMPTS[1:]
+    lens = [a + n for a, n in prompts]
+    k, v, table = make_cache(g, lens, 32, 2, 128, torch.bfloat16)
+    total = sum(n for _, n in prompts)
+    cu = [sum(n for _, n in prompts[:r]) for r in range(len(prompts) + 1)]
+    q = (0.2 * torch.randn(total, 40, 128, generator=g, device=DEV)).to(torch.bfloat16)
+    call = lambda: pkg.paged_attention_prefill(q, k, v, ints(table), ints(lens), ints(cu), max_len=max_len)
+    before = call()
+    v[table[9][100 // 32], :, 100 % 32, 5] = float("inf")     # the request of 200 tokens: rows 100 .. see it
+    q[cu[4] + 3] = NAN                                        # a row of the request of 65
+    after = call()
+    rows = torch.ones(total, dtype=torch.bool, device=DEV)
+    rows[cu[9] + 100:cu[10]] = False
+    rows[cu[4] + 3] = False
+    assert torch.isfinite(after[rows].float()).all()
+    assert float((after[rows].float() - before[rows].float()).abs().max()) < 0.02     # (rows summed again in 32 bits)
+    assert bool((after[cu[9] + 100:cu[10], :, 5] == float("inf")).all()) and bool(after[cu[4] + 3].isnan().all())
+    rest = [d for d in range(128) if d != 5]
+    assert torch.isfinite(after[cu[9] + 100:cu[10]][:, :, rest].float()).all()
+
+
 def test_prefill_many_requests(pkg):
     """More requests than a wave's lanes, most of them with a token or none."""
     prompts = [(r % 7, r % 3) for r in range(150)] + [(20, 140)]
