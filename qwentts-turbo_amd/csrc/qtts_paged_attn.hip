@@ -64,8 +64,9 @@ __device__ __forceinline__ Blocks blocks_of(int lo, int end, int sinks) {
 
 // Staged rows: row r of a block at r * 2 D bytes, its 16-byte chunk c at position c ^ swz(r). LDS serves 256 bytes
 // a cycle from 64 banks; with this permutation the 16 rows of an operand read (one chunk each) and the 4 rows x
-// 64 bytes of a transpose read fall on different banks (with c ^ (r & 7) the transpose reads of 4 rows fell on the
-// same 64 bytes: two thirds of the LDS cycles were conflicts).
+// 64 bytes of a transpose read of the prefill fall on different banks (with c ^ (r & 7) the transpose reads of 4 rows
+// fell on the same 64 bytes: two thirds of the LDS cycles were conflicts; now none are). The decode's transpose reads, 8
+// rows x 32 bytes, meet two at a time; a permutation for them changed no time (its LDS is busy 16% of the cycles).
 template <int D>
 __device__ __forceinline__ int swz(int r) {
   if constexpr (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
@@ -117,6 +118,10 @@ struct PieceCopy {
 //     16 + 4 g + j - 4 above), V^T comes through LDS transpose reads of 4 keys each. P goes in as two 16-bit
 //     numbers, the rounded value and the rounded rest, so that its rounding is that of 16 bits or more: the
 //     matrix units are idle otherwise.
+// Measured (us, and of K and V read): 64 requests of 129 to 4090 keys, 16 / 8 heads of 128, bf16 97 with the join (5.65
+// TB/s; reading that much does 7.0), 24 under a window of 1024 20.3 (5.0), 3 of 40000 to 60000 keys, 32 / 4 heads of
+// 64, fp16 32 (5.0); one of 700 keys 10.0: two launches and the chain lengths -> table -> K -> scores -> V -> join. What
+// the long ones lose against a plain read is each unit's beginning and end, where its 64 KB are not in flight.
 // The heads of a group share every K and V byte; a group over 16 is several workgroups. The waves join through
 // LDS, the units of a request through part / part_ml and decode_join_kernel, both in key order, so results do not
 // depend on timing. A request of one unit writes its output here.
@@ -441,7 +446,7 @@ __global__ void __launch_bounds__(64 * W, 2) decode_kernel(const AttnArgs g) {
   }
 }
 
-// The units of a request's head joined: one workgroup per (request, query head), its D / 4 lanes a unit taking 4
+// The units of a request's head joined (3 to 5 us, a dependent launch): one workgroup per (request, query head), its D / 4 lanes a unit taking 4
 // channels each and its groups of lanes units u, u + groups, ..; the groups' sums add through LDS in order. Loads do
 // not wait for the request's length (what a unit past its last has in its place is passed over), so the chain is one
 // read, not three.
@@ -515,8 +520,12 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const AttnArgs g) {
 //   S^T = K Q^T on MFMA 32x32x16 (A: 32 keys from LDS, B: the rows in registers): lane (hf, c) holds row c's
 //     scores of keys 8 (r >> 2) + 4 hf + (r & 3), so a row's max and sum are in-lane and one exchange.
 //   O^T += V^T P^T with the score registers as P^T (k-index 8 hf + j of step kk is key 16 kk + 8 (j >> 2) +
-//     4 hf + (j & 3)) and V^T by LDS transpose reads. P is rounded to the element type, as V is; its sum
-//     is of the unrounded values in f32.
+//     4 hf + (j & 3)) and V^T by LDS transpose reads. P is rounded to the element type, as V is (in two
+//     parts, as in decode, it would cost half as many matrix products again); its sum is of the unrounded values in f32.
+// Bound by the issue of matrix products (34% of the SIMDs' cycles) and vector instructions (40%), with two waves a SIMD to
+// run one under the other; with 64 channels the exponentials and masks take 65%. Measured: a prompt of 4096 tokens, 16 / 8
+// heads of 128, bf16 82 us (840 TFLOP/s; a large library product does 1208), 3 of 1111 to 3500 under a window of 777,
+// 32 / 4 heads of 64, fp16 86 (580), 12 of 5 to 300 tokens after up to 900 25.7, two rounds of tiles.
 // The running max moves only when a row's block max passes it by more than a factor 2^8 of the weights. The
 // splits of a row join through LDS in key order.
 // A weight that is masked is 0, but 0 times an infinite or NaN v_j is NaN, and a key may be hidden from one
@@ -671,8 +680,8 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
     const int page = __builtin_amdgcn_readlane(x.e, w % NP), none = (int)((has >> (w % NP)) & 1) - 1;   // -1: none
     return page | none;
   };
-  // steps whose wave's block is seen whole by all its rows, and whose copies (this wave's pieces of V a step and of K
-  // two steps on) are whole: no mask, no partial piece
+  // steps whose wave's block is seen whole by all its rows, and whose copies (of the next step's K
+  // and V) are whole: no mask, no partial piece
   int fs, fe;
   {
     const int see0 = g.window > 0 ? max(bl.ns, (max(whi - g.window + 1, 0) + KB - 1) / KB - bl.skip) : 0;
@@ -824,7 +833,7 @@ __global__ void __launch_bounds__(64 * PWV, D == 128 ? 2 : 4) prefill_kernel(con
       sum += e0;
       sum += e1;
       p[j >> 2][j & 3] = E::pack(e0, e1);
-      // one copy at a time between the exponentials: issued together they hold the wave for 130 cycles each
+      // one copy at a time between the exponentials: issued together each holds the wave for 130 cycles
       constexpr int every = 8 * NU / (PAIR * copy.N);
       if (j % every == every - 1) {
         const int n = j / every;
@@ -1036,6 +1045,7 @@ hipError_t launch_prefill(const AttnArgs& g, hipStream_t st) {
   hipLaunchKernelGGL((prefill_kernel<E, D, NS>), dim3((unsigned)(tiles * g.hkv)), dim3(64 * PWV), 0, st, g);
   return hipGetLastError();
 }
+
 // Which tiles: 256 rows unsplit (NS = 1) take the fewest key steps for all the rows together, 64 rows in 4 key splits
 // the shortest chain for one tile. A launch takes the longer of the longest tile's chain and all tiles' steps over
 // the tiles that run at once (one a CU with 128 channels, two with 64), estimated with 2 to 2.5 us a tile and
