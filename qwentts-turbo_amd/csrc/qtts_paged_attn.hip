@@ -66,7 +66,7 @@ __device__ __forceinline__ Blocks blocks_of(int lo, int end, int sinks) {
 // a cycle from 64 banks; with this permutation the 16 rows of an operand read (one chunk each) and the 4 rows x
 // 64 bytes of a transpose read of the prefill fall on different banks (with c ^ (r & 7) the transpose reads of 4 rows
 // fell on the same 64 bytes: two thirds of the LDS cycles were conflicts; now none are). The decode's transpose reads, 8
-// rows x 32 bytes, meet two at a time; a permutation for them changed no time (its LDS is busy 16% of the cycles).
+// rows x 32 bytes, meet two at a time; a permutation for them changed no time (its LDS is busy 15% of the cycles).
 template <int D>
 __device__ __forceinline__ int swz(int r) {
   if constexpr (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
