@@ -5,6 +5,8 @@ A = sum p |v|: f32 scores (128 products: 128 * 2^-24 of scale * sum |q k|, about
 weight and as much of their sum), sums over up to 2,500 keys in f32 chains of at most 1,250 (7.5e-5), and the hardware's
 exp2 (2^-22): 3e-4 A covers them. Prefill rounds the weights to the type: eps / 2 of A more. The norm and rotation
 are a dozen f32 operations on values below the head's norm: 1e-5 of max |y| covers them."""
+import math
+
 import pytest
 import torch
 
@@ -387,6 +389,27 @@ def test_large_scores_and_scale(pkg):
     # scores up to 2^13: f32 steps of 2^-10 each, 128 products: weights off by at most e^(128 * 2^-11) - 1 = 6.5 %
     for a, b in ((out, ref), (one, ref[299:])):
         assert torch.isfinite(a).all() and float((a.double() - b).abs().max()) < 0.065 * float(v[~v.isnan()].abs().max())
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float16, 64), (torch.float16, 128), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("max_len", [1, 8001])
+def test_many_small_weights(pkg, dtype, dim, max_len):
+    """One key of weight 1 and 8000 of 4e-5 (below fp16's normal numbers): together they weigh a fourth, and V is 1 for
+    the one and 2 for the others."""
+    n = 8001
+    table = [list(range(-(-n // 16)))]
+    k = torch.zeros(len(table[0]), 1, 16, dim, device=DEV, dtype=dtype)
+    v = torch.full_like(k, 2.0)
+    k[70, 0, 5, 0], v[70, 0, 5] = 1.0, 1.0
+    q = torch.zeros(2, 3, dim, device=DEV, dtype=dtype)
+    q[:, :, 0] = 10.125                                       # e^-10.125 = 4.006e-5
+    w = 8000 * math.exp(-10.125)
+    one = pkg.paged_attention_decode(q[:1], k, v, ints(table), ints([n]), scale=1.0)
+    two = pkg.paged_attention_prefill(q[:1], k, v, ints(table), ints([n]), ints([0, 1]), scale=1.0, max_len=max_len)
+    # the output's half step, and a weight's rounding (4e-5 in fp16: steps of 2^-24, 7.4e-4 of it at most) in its share
+    tol = half(dtype) * 2 + (7.5e-4 if dtype == torch.float16 else half(dtype)) * w / (1 + w) * 2 + 3e-4
+    for out in (one, two):
+        assert float((out.double() - (1 + 2 * w) / (1 + w)).abs().max()) < tol
 
 
 def test_strides_and_tables(pkg):
