@@ -36,6 +36,7 @@ struct AttnArgs {
   int requests, tokens, hq, hkv, group;          // group: query heads of a KV head
   float scale_log2;                              // scale * log2(e)
   int window, sinks;                             // window 0: none
+  int merged;                                    // prefill: tiles of all requests in one order (find_tile)
   int splits, blocks;                            // decode: most units of a request, blocks a unit
   float* part;                                   // [requests][hq][splits][D] sums
   float* part_ml;                                // [requests][hq][splits][2] running max and sum
@@ -580,8 +581,10 @@ __device__ __forceinline__ void exact_row(const AttnArgs& g, int b, int kvh, int
   else *op = (uint16_t)E::pack(x * rl, 0.0f);
 }
 
-// A tile of PM rows over all requests, counted from the last back (the longest keys first): its request and its
-// place in it; request -1 past the first. Every lane takes a request, 64 at a time.
+// Tile number `back` of PM rows, the longest keys first: its request and its place in it; request -1 past the last
+// one. Either request by request from the last, every lane taking a request, 64 at a time; or (merged, up to 64
+// requests) over all of them: a request's tiles lie at the places ceil(len group / PM) and downwards, one each, and the
+// place of number `back` is found by halving on how many tiles lie past it.
 struct TilePlace {
   int b, tile, first, n;              // request, tile in it, first token, tokens
 };
@@ -599,6 +602,45 @@ __device__ __forceinline__ int tiles_of(const AttnArgs& g, int b, int* first, in
 template <int PM>
 __device__ __forceinline__ TilePlace find_tile(const AttnArgs& g, int back) {
   const int lane = threadIdx.x & 63;
+  if (g.merged) {
+    int first, n;
+    const int own = tiles_of<PM>(g, lane, &first, &n);
+    const int len = request_len(g, min(lane, g.requests - 1));
+    const int top = (int)min(((long long)len * g.group + PM - 1) / PM, 1ll << 29);   // place of the request's last tile
+    auto most = [](int x) QTTS_PG_INLINE {
+      x = max(x, (int)xlane<0>((uint32_t)x));
+      x = max(x, (int)xlane<1>((uint32_t)x));
+      x = max(x, (int)xlane<2>((uint32_t)x));
+      x = max(x, (int)xlane<3>((uint32_t)x));
+      x = max(x, (int)xlane<4>((uint32_t)x));
+      return __builtin_amdgcn_readfirstlane(max(x, (int)xlane<5>((uint32_t)x)));
+    };
+    auto behind = [&](int place) QTTS_PG_INLINE {        // tiles of all requests past a place
+      int x = min(max(top - place, 0), own);
+      x += (int)xlane<0>((uint32_t)x);
+      x += (int)xlane<1>((uint32_t)x);
+      x += (int)xlane<2>((uint32_t)x);
+      x += (int)xlane<3>((uint32_t)x);
+      x += (int)xlane<4>((uint32_t)x);
+      return __builtin_amdgcn_readfirstlane(x + (int)xlane<5>((uint32_t)x));
+    };
+    int lo = -most(own > 0 ? own - top : -(1 << 30)), up = most(own > 0 ? top : -(1 << 30));   // lo: before every tile
+    if (up < lo || back >= behind(lo)) return TilePlace{-1, 0, 0, 0};
+    while (lo < up) {                                    // the least place with at most `back` tiles past it
+      const int mid = lo + ((up - lo) >> 1);
+      if (behind(mid) <= back) up = mid;
+      else lo = mid + 1;
+    }
+    const uint64_t here = __builtin_amdgcn_ballot_w64((top >= lo) & (top - lo < own));
+    const int rank = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(here >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)here, 0u));
+    const int src = __builtin_ctzll(here & __builtin_amdgcn_ballot_w64(rank == back - behind(lo)));
+    TilePlace p;
+    p.b = src;
+    p.tile = __builtin_amdgcn_readlane(own, src) - 1 - (__builtin_amdgcn_readlane(top, src) - lo);
+    p.first = __builtin_amdgcn_readlane(first, src);
+    p.n = __builtin_amdgcn_readlane(n, src);
+    return p;
+  }
   for (int b0 = (g.requests - 1) & ~63; b0 >= 0; b0 -= 64) {
     int first, n;
     const int own = tiles_of<PM>(g, b0 + lane, &first, &n);
@@ -1053,10 +1095,18 @@ hipError_t launch_prefill(const AttnArgs& g, hipStream_t st) {
 // a prompt of 300 tokens 16.4 : 14.4 : 11.6, 1000 35.6 : 23.7 : 18.0, 2000 61.3 : 39.4 : 37.5, 4096 117.8 : 89.5 : 114.5,
 // 8192 278.8 : 294.8 : 366; 64 prompts of 20 to 100 25.5 : 36.1 : 40.9; 8 of 50 to 100 after 4000 104 : 57 : 44; 8192 under
 // a window of 512 77 : 81 : 107.
+// Merged order (find_tile): where a tile's keys grow with its place and the longest tile is more than half of what all take;
+// its start costs 0.5 us, and it reads more requests' keys at once (us, merged : not: 4 prompts of 2000 91 : 117, 16 of 500
+// 43.5 : 51.8, 6 of 100 to 3000 115 : 130, 16 of 100 to 200, 32 / 4 heads of 64, 15.2 : 16.5; but 40 of 300 67 : 62, 3 under a
+// window 100 : 95, 8 pieces of up to 512 after 4000 60.5 : 58.7).
+struct Tiles {
+  int splits;
+  bool merged;
+};
 template <int D>
-int prefill_splits(const AttnArgs& g, int max_len) {
+Tiles prefill_tiles(const AttnArgs& g, int max_len) {
   const double each = (double)g.tokens / g.requests, slots = D == 128 ? 256 : 512;
-  int pick = 1;
+  Tiles pick{1, false};
   double best = 1e30;
   for (int ns = 1; ns <= 4; ns *= 2) {
     const int pm = 32 * PWV / ns, step = ns == 4 ? 128 : 64 * ns;
@@ -1067,17 +1117,19 @@ int prefill_splits(const AttnArgs& g, int max_len) {
       longest = std::min(longest, span);
       mean = std::min(mean, span);
     }
-    const double t = std::max(tile + std::ceil(longest / step) * cost, n / slots * (tile + std::ceil(mean / step) * cost));
-    if (t < best) {
-      best = t;
-      pick = ns;
+    const double chain = tile + std::ceil(longest / step) * cost, all = n / slots * (tile + std::ceil(mean / step) * cost);
+    if (std::max(chain, all) < best) {
+      best = std::max(chain, all);
+      pick = Tiles{ns, g.requests > 1 && g.requests <= 64 && longest > 1.25 * mean && 2 * chain > all};
     }
   }
   return pick;
 }
 template <class E, int D>
-hipError_t launch_prefill_any(const AttnArgs& g, int max_len, hipStream_t st) {
-  switch (prefill_splits<D>(g, max_len)) {
+hipError_t launch_prefill_any(AttnArgs& g, int max_len, hipStream_t st) {
+  const Tiles t = prefill_tiles<D>(g, max_len);
+  g.merged = t.merged ? 1 : 0;
+  switch (t.splits) {
     case 1: return launch_prefill<E, D, 1>(g, st);
     case 2: return launch_prefill<E, D, 2>(g, st);
     default: return launch_prefill<E, D, 4>(g, st);

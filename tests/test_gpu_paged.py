@@ -291,6 +291,25 @@ def test_prefill_many_requests(pkg):
     run_prefill(pkg, prompts, 16, 8, 128, torch.bfloat16, 16, "heads_first", 0, 0)
 
 
+@pytest.mark.parametrize("prompts", [[(0, 400)] * 3 + [(0, 0), (0, 7), (2, 333)], [(0, 1)] * 30 + [(0, 0)] * 20 + [(0, 300)] * 14,
+                                     [(0, 90), (0, 0), (0, 700)]])
+@pytest.mark.parametrize("hq,hkv,dim,dtype", [(16, 8, 128, torch.bfloat16), (9, 3, 64, torch.float16)])
+def test_prefill_tiles_of_many_requests_in_one_order(pkg, prompts, hq, hkv, dim, dtype):
+    """Prompts whose keys grow with their tiles: the longest tiles of all of them first. Lengths shorter than the tokens
+    and padding beside them."""
+    run_prefill(pkg, prompts, hq, hkv, dim, dtype, 16, "tokens_first", 0, 0, max_len=max(a + n for a, n in prompts))
+    n = 150
+    g = gen(8)
+    k, v, table = make_cache(g, [n, n, n, n], 16, hkv, dim, dtype)
+    q = torch.randn(4 * n + 5, hq, dim, generator=g, device=DEV).to(dtype)
+    lens, cu = [n, 0, 40, n], [0, n, 2 * n, 3 * n, 4 * n]     # a refused request, one shorter than its tokens
+    out = pkg.paged_attention_prefill(q, k, v, ints(table), ints(lens), ints(cu), max_len=n, out=torch.full_like(q, 5.0))
+    pos = [lens[r] - n + i for r in range(4) for i in range(n)]
+    ref, mag = oracle.attend(q[:4 * n], k, v, [table[r] for r in range(4) for _ in range(n)], pos, hq // hkv, 0, 0, dim ** -0.5)
+    check(out[:4 * n], ref, mag, dtype, True)
+    assert bool((out[4 * n:] == 5.0).all())
+
+
 def test_prefill_longer(pkg):
     run_prefill(pkg, [(700, 600), (0, 333)], 4, 2, 128, torch.bfloat16, 32, "heads_first", 0, 0)
     run_prefill(pkg, [(1500, 40)], 4, 2, 64, torch.float16, 32, "heads_first", 200, 9)
