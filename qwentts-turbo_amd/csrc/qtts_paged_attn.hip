@@ -1051,18 +1051,21 @@ AttnArgs attn_args(const QttsPagedCache* cache, int hq, const void* q, long long
 // and end (us, unsplit against units of 512 keys: 200 requests of 100 to 700 keys 59.5 : 88.9, 64 of 50 to 300
 // 13.3 : 22.7 (256 keys); 24 under a window of 1024 21.6 : 26.5), but 64 ragged ones up to 4090 keys leave a shorter last
 // round (101.8 : 108.8, 16 up to 4000 31.0 : 33.5). Fewer pairs are split down to 256 keys a unit, until there
-// are 512 units (one request of 700 keys 9.8 : 10.1 unsplit, of 2000 10.7 : 21.7, of 60000 in 512 units 46.7, in 1024
-// 49.8).
+// are 512 units (one request of 1000 keys 10.0 : 11.5 unsplit, of 2000 10.7 : 21.7, of 60000 in 512 units 46.7, in 1024
+// 49.8). Up to 512 keys 8 waves take them unsplit (one of 300 to 512 9.0 : 10.0, 4 10.3 : 10.8), up to 768 those of 64
+// channels (700 keys 8.6 : 9.7, 300 6.3 : 9.4) or of 64 pairs (12 requests of 700 14.7 : 16.4, but of 1000 19.0 : 17.5); up
+// to 256 keys 4 waves do (6.5, 8 waves 7.1).
 struct Split {
   int splits, blocks;      // most units, blocks a unit
-  bool wide;               // 8 waves a workgroup: for unsplit pairs that leave a CU one workgroup
+  bool wide;               // 8 waves a workgroup, where a CU has one
 };
-Split decode_split(int requests, int hkv, int group, int width, int page_size, int max_len, int window, int sinks) {
+Split decode_split(int requests, int hkv, int group, int head_dim, int width, int page_size, int max_len, int window, int sinks) {
   long long keys = std::min<long long>((long long)width * page_size, max_len);
   if (window > 0) keys = std::min<long long>(keys, (long long)window + std::min<long long>(sinks, keys) + 2 * DKB);
   const long long blocks = std::max<long long>(1, (keys + DKB - 1) / DKB);
   const long long pairs = (long long)requests * hkv * ((group + 15) / 16);
   if (pairs >= 128 && blocks < 64) return Split{1, (int)blocks, pairs <= 256};
+  if (pairs < 128 && blocks <= (head_dim == 64 || pairs >= 64 ? 24 : 16)) return Split{1, (int)blocks, blocks > 8};
   const long long units = pairs >= 128 ? 4096 : 512, least = pairs > 256 ? 16 : 8;
   long long per = std::max(least, (blocks * pairs + units - 1) / units);
   per = std::min((per + 3) / 4 * 4, blocks);
@@ -1149,7 +1152,7 @@ size_t qtts_paged_decode_workspace_bytes(int n_requests, int num_q_heads, int nu
   if (n_requests < 1 || num_kv_heads < 1 || num_q_heads < 1 || num_q_heads % num_kv_heads != 0 || head_dim < 1 ||
       table_width < 1 || page_size < 1 || max_len < 1 || window < 0 || sinks < 0)
     return 0;
-  const Split s = decode_split(n_requests, num_kv_heads, num_q_heads / num_kv_heads, table_width, page_size, max_len, window, sinks);
+  const Split s = decode_split(n_requests, num_kv_heads, num_q_heads / num_kv_heads, head_dim, table_width, page_size, max_len, window, sinks);
   return s.splits == 1 ? 0 : (size_t)n_requests * num_q_heads * s.splits * (head_dim + 2) * 4;
 }
 
@@ -1164,7 +1167,7 @@ hipError_t qtts_paged_attention_decode(const QttsPagedCache* cache, int n_reques
     return hipErrorInvalidValue;
   AttnArgs g = attn_args(cache, num_q_heads, q, q_token_stride, q_head_stride, out, out_token_stride, out_head_stride,
                          block_table, table_width, table_stride, kv_lens, n_requests, scale, window, sinks);
-  const Split s = decode_split(n_requests, g.hkv, g.group, table_width, cache->page_size, max_len, window, sinks);
+  const Split s = decode_split(n_requests, g.hkv, g.group, cache->head_dim, table_width, cache->page_size, max_len, window, sinks);
   g.splits = s.splits;
   g.blocks = s.blocks;
   if (s.splits > 1) {
