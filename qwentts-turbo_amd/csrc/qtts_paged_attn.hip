@@ -447,10 +447,10 @@ __global__ void __launch_bounds__(64 * W, 2) decode_kernel(const AttnArgs g) {
   }
 }
 
-// The units of a request's head joined (3 to 5 us, a dependent launch): one workgroup per (request, query head), its D / 4 lanes a unit taking 4
-// channels each and its groups of lanes units u, u + groups, ..; the groups' sums add through LDS in order. Loads do
-// not wait for the request's length (what a unit past its last has in its place is passed over), so the chain is one
-// read, not three.
+// The units of a request's head joined (3 to 5 us, a dependent launch): one workgroup per (request, query head), its
+// D / 4 lanes a unit taking 4 channels each and its groups of lanes units u, u + groups, ..; the groups' sums add
+// through LDS in order. Loads do not wait for the request's length (what a unit past its last has in its place is
+// passed over), so the chain is one read, not three.
 template <class E, int D>
 __global__ void __launch_bounds__(256) decode_join_kernel(const AttnArgs g) {
   constexpr int LU = D / 4, GR = 256 / LU, AT = 4;   // lanes a unit, groups, units of a group read at once
@@ -1053,8 +1053,8 @@ AttnArgs attn_args(const QttsPagedCache* cache, int hq, const void* q, long long
 // round (101.8 : 108.8, 16 up to 4000 31.0 : 33.5). Fewer pairs are split down to 256 keys a unit, until there
 // are 512 units (one request of 1000 keys 10.0 : 11.5 unsplit, of 2000 10.7 : 21.7, of 60000 in 512 units 46.7, in 1024
 // 49.8). Up to 512 keys 8 waves take them unsplit (one of 300 to 512 9.0 : 10.0, 4 10.3 : 10.8), up to 768 those of 64
-// channels (700 keys 8.6 : 9.7, 300 6.3 : 9.4) or of 64 pairs (12 requests of 700 14.7 : 16.4, but of 1000 19.0 : 17.5); up
-// to 256 keys 4 waves do (6.5, 8 waves 7.1).
+// channels (700 keys 8.6 to 9.0 : 9.7, 300 6.3 to 6.8 : 9.4) or of 64 pairs (12 requests of 700 14.7 : 16.4, but of 1000
+// 19.0 : 17.5); up to 256 keys 4 waves do (6.5, 8 waves 7.1).
 struct Split {
   int splits, blocks;      // most units, blocks a unit
   bool wide;               // 8 waves a workgroup, where a CU has one
