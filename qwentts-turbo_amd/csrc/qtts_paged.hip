@@ -22,8 +22,7 @@ namespace pg {
 // tokens as flat lists, each element finding its request by a search in LDS. It is bound by latency: the chain is
 // lengths -> sums -> free pages -> slots; 256 threads for up to 256 requests, whose sums cross 4 waves and not 16
 // (64 requests of one token 4.1 us, 7.1 on 16 waves). Measured: 64 requests 6.1 us a call, of which an empty launch is
-// 2 to 3; 400 requests with 60 prompts up to 1500 tokens 11.8 (this kernel 7.2, the tokens 4.7: a search through the
-// requests' sums for each).
+// 2 to 3; 400 requests with 60 prompts up to 1500 tokens 10.9 (this kernel 7.2, the tokens 4.0).
 constexpr int PT = 1024;
 
 // Inclusive prefix sums of N values over the workgroup of NT threads; total[] receives the sums. `part`: N * NT / 64
@@ -177,13 +176,22 @@ __global__ void __launch_bounds__(NT) plan_kernel(const PlanArgs g) {
   if (t == 0) *g.free_out = (int)(free_n - s_given);
 }
 
-// The tokens of a large plan, from what plan_kernel left: one thread a token over the whole GPU.
+// The tokens of a large plan, from what plan_kernel left: one thread a token over the whole GPU. Its chain is the search,
+// a step a load; up to 2048 requests' sums come into LDS first, two loads deep (400 requests: a call 10.9 us, 11.8 when
+// it searched them in memory).
+constexpr int PL = 2048;
 __global__ void __launch_bounds__(256) plan_tokens_kernel(const PlanArgs g) {
+  __shared__ int s_cu[PL];
   const int q = blockIdx.x * 256 + threadIdx.x;
+  const bool in_lds = g.n <= PL;
+  if (in_lds) {
+    for (int i = threadIdx.x; i < g.n; i += 256) s_cu[i] = g.cu[i + 1];
+    __syncthreads();
+  }
   if (q >= g.total) return;
   int slot = -1, pos = 0;
-  if (q < g.cu[g.n]) {
-    const int r = first_above(g.cu + 1, g.n, q);
+  if (q < (in_lds ? s_cu[g.n - 1] : g.cu[g.n])) {
+    const int r = in_lds ? first_above(s_cu, g.n, q) : first_above(g.cu + 1, g.n, q);
     const int i = q - g.cu[r];
     if (g.status[r] == 0) {
       pos = g.lengths_out[r] - (g.cu[r + 1] - g.cu[r]) + i;
